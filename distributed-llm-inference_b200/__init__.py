@@ -11,6 +11,13 @@ Public ops (drop-in for the reference's decode path):
       one decode layer (RoPE, slot writes, attention) in one launch
   prefill_attention(q, k_pool, v_pool, tables, lengths)
       causal prefill attention with K/V from the pools (worker/llama.py:141-144)
+  shared_prefix_attention(q, k, v, prefix_table, prefix_length, tables, lengths, max_length)
+      attention of a batch that shares a prefix; several (drafted) tokens per
+      sequence, optional accumulated attention weights
+  verify_drafts(draft_tokens, target_probs, accept_uniforms, sample_uniforms)
+      accepts drafted tokens and draws the next one
+  evict_tokens(k, v, scores, tables, lengths, new_tables, budget, recent)
+      keeps a cache under a budget by accumulated weight
   DevicePagedKV              TensorPagedKV (worker/llama.py:13-55) + device-resident
                              decode tables/lengths
   PagedLlama                 worker/llama.py:89-177 on these ops (CUDA-graph decode ticks)
@@ -25,11 +32,14 @@ from ._lib import PREFILL_AUTO, PREFILL_MMA, PREFILL_TCGEN05  # noqa: F401
 from .ops import (decode_attention, decode_attention_supported,  # noqa: F401
                   fast_grid_size, paged_attention, prefill_attention, read_device_errors,
                   rope_kv_write, rope_kv_write_decode)
+from ._lib import PREFIX_AUTO, PREFIX_SIMT  # noqa: F401
+from .serving_ops import evict_tokens, shared_prefix_attention, verify_drafts  # noqa: F401
 from .paged_kv import DevicePagedKV  # noqa: F401
 from .llama_runner import PagedLlama  # noqa: F401
 from .integration import cuda_paged_attention, install, uninstall  # noqa: F401
 
 __all__ = [
+    "shared_prefix_attention", "verify_drafts", "evict_tokens",
     "paged_attention", "decode_attention", "decode_attention_supported", "prefill_attention",
     "rope_kv_write", "rope_kv_write_decode",
     "DevicePagedKV", "PagedLlama",

@@ -56,6 +56,18 @@ SIGNATURES = {
                                           _c_ptr, _c_i64, _c_ptr, _c_int, _c_ptr, _c_i64,
                                           _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int,
                                           _c_ptr]),
+    "pdb_shared_prefix_attention": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64,
+                                             _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64,
+                                             _c_ptr] + [_c_i64] * 9 + [_c_int, _c_ptr, _c_size,
+                                                                       _c_ptr]),
+    "pdb_shared_prefix_attention_impl": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64,
+                                                  _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64,
+                                                  _c_ptr] + [_c_i64] * 9
+                                         + [_c_int, _c_ptr, _c_size, _c_ptr, _c_int]),
+    "pdb_shared_prefix_attention_workspace_size": (_c_size, [_c_i64] * 7 + [_c_int, _c_int]),
+    "pdb_verify_drafts": (_c_int, [_c_ptr] * 8 + [_c_i64] * 3 + [_c_int, _c_ptr]),
+    "pdb_evict_tokens": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64] + [_c_ptr] * 6 + [_c_i64] * 9
+                         + [_c_int, _c_ptr]),
     "pdb_read_device_errors": (_c_int, [ctypes.POINTER(ctypes.c_uint32), _c_int]),
     "pdb_debug_partition": (_c_i64, [_c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr]),
     "pdb_debug_dyn_partition": (_c_i64, [_c_i64, _c_i64, _c_ptr, _c_i64]),
@@ -66,6 +78,7 @@ DTYPE_FLOAT32 = 0
 DTYPE_FLOAT16 = 1
 IMPL_AUTO, IMPL_FAST, IMPL_GENERIC, IMPL_SIMT, IMPL_MMA, IMPL_TMA_STATIC = 0, 1, 2, 3, 4, 5
 PREFILL_AUTO, PREFILL_TCGEN05, PREFILL_MMA = 0, 1, 2
+PREFIX_AUTO, PREFIX_SIMT = 0, 1
 DECODE_STABLE_METADATA = 0x1
 DECODE_STABLE_POOLS = 0x2
 STATUS_NAMES = {0: "ok", 1: "invalid argument", 2: "workspace", 3: "cuda"}

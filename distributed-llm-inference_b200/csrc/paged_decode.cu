@@ -1143,3 +1143,5 @@ int64_t pdb_debug_partition(const int32_t* lengths, int64_t batch, int64_t kv_he
 }
 
 }  // extern "C"
+
+#include "serving_ops.cuh"

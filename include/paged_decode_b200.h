@@ -71,6 +71,12 @@ typedef enum {
   PDB_PREFILL_MMA = 2      /* cp.async-staged tiles, mma.sync, any block size        */
 } pdb_prefill_impl_t;
 
+/* Kernel selection for pdb_shared_prefix_attention_impl. */
+typedef enum {
+  PDB_PREFIX_AUTO = 0, /* by shape                                              */
+  PDB_PREFIX_SIMT = 1  /* FP32 arithmetic throughout, any shape                 */
+} pdb_prefix_impl_t;
+
 /* Bits of the per-device error word (pdb_read_device_errors). */
 #define PDB_DEVERR_TABLE_ENTRY 0x1u  /* block-table entry outside [0, num_blocks) */
 #define PDB_DEVERR_LENGTH 0x2u       /* length < 0 or > table_width*block_size   */
@@ -80,6 +86,7 @@ typedef enum {
                                         expired (never expected; see kernel notes) */
 #define PDB_DEVERR_ARRIVAL 0x20u     /* a piece could not register its arrival
                                         (never expected)                          */
+#define PDB_DEVERR_TOKEN 0x40u       /* drafted token outside the vocabulary      */
 
 /* Thread-local message of the last failed call ("" if none). */
 PDB_API const char* pdb_last_error(void);
@@ -356,6 +363,114 @@ PDB_API int64_t pdb_debug_dyn_partition(int64_t units, int64_t launched, int64_t
  * shape (0 when the fast kernel does not apply). No reference counterpart. */
 PDB_API int64_t pdb_fast_grid_size(int64_t batch, int64_t heads, int64_t kv_heads,
                            int64_t head_dim, int dtype);
+
+/*
+ * Attention of a batch whose sequences share a long prefix: the prefix's K and
+ * V are read once for all of them. No reference counterpart (its decode reads
+ * every sequence's whole context).
+ *   q, out   [batch, tokens, heads, head_dim]: `tokens` >= 1 query tokens per
+ *            sequence (1 in a decode step; the drafted tokens of a speculative one)
+ *   k_pool, v_pool [num_blocks, block_size, kv_heads, head_dim]
+ *   prefix_table int32 [prefix_pages], the prefix's pages; its first
+ *            prefix_length tokens are seen by every query token (0: no prefix)
+ *   tables   int32 [batch, table_width], sequence b's own pages
+ *   lengths  int32 [batch], its own cached tokens, the new ones included
+ *            (<= max_length <= table_width * block_size)
+ *   counts   int32 [batch] or NULL: how many of the query tokens are real
+ *            (NULL: all). Token t < counts[b] is the sequence's own token
+ *            lengths[b] - counts[b] + t: it sees the prefix and own tokens up
+ *            to itself. Rows t >= counts[b] and rows that see nothing are 0.
+ *   scores, scores_out fp32 [batch, kv_heads, scores_width] or both NULL:
+ *            scores_out[b][c][j] = scores[b][c][j] + the softmax weight that
+ *            own token j got from the real query tokens and the heads of kv
+ *            head c, summed (unchanged for j >= lengths[b]). May be the same
+ *            buffer. scores_width >= max_length.
+ * Query head h reads kv head h / (heads / kv_heads); scale 1 / sqrt(head_dim).
+ * FP16: products on tensor cores, sums and softmax statistics in FP32.
+ * Lengths and counts out of range are clamped, pages out of range read as
+ * zeros; both set device error bits. Results do not depend on timing.
+ * Capturable. The workspace is 256-byte aligned, of
+ * pdb_shared_prefix_attention_workspace_size bytes; contents do not matter.
+ */
+PDB_API int pdb_shared_prefix_attention(
+    const void* q, const void* k_pool, const void* v_pool, const int32_t* prefix_table,
+    int64_t prefix_pages, int64_t prefix_length, const int32_t* tables, const int32_t* lengths,
+    const int32_t* counts, const float* scores, float* scores_out, int64_t scores_width, void* out,
+    int64_t batch, int64_t tokens, int64_t heads, int64_t head_dim, int64_t num_blocks,
+    int64_t block_size, int64_t kv_heads, int64_t table_width, int64_t max_length, int dtype,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same with the kernels pinned (pdb_prefix_impl_t), for tests. */
+PDB_API int pdb_shared_prefix_attention_impl(
+    const void* q, const void* k_pool, const void* v_pool, const int32_t* prefix_table,
+    int64_t prefix_pages, int64_t prefix_length, const int32_t* tables, const int32_t* lengths,
+    const int32_t* counts, const float* scores, float* scores_out, int64_t scores_width, void* out,
+    int64_t batch, int64_t tokens, int64_t heads, int64_t head_dim, int64_t num_blocks,
+    int64_t block_size, int64_t kv_heads, int64_t table_width, int64_t max_length, int dtype,
+    void* workspace, size_t workspace_bytes, void* stream, int impl);
+
+/* Workspace bytes of pdb_shared_prefix_attention for this shape (any kernel). */
+PDB_API size_t pdb_shared_prefix_attention_workspace_size(int64_t batch, int64_t tokens,
+                                                          int64_t heads, int64_t kv_heads,
+                                                          int64_t head_dim, int64_t prefix_length,
+                                                          int64_t max_length, int dtype,
+                                                          int with_scores);
+
+/*
+ * Verification of drafted tokens against the target's probabilities. No
+ * reference counterpart (it decodes one token per step).
+ *   draft_tokens int64 [batch, drafts]; draft_lengths int32 [batch] or NULL
+ *            (all): sequence b drafted its first draft_lengths[b] tokens
+ *   target_probs [batch, drafts + 1, vocab], draft_probs [batch, drafts,
+ *            vocab] or NULL (tokens that were not sampled: probability 1 at
+ *            the drafted token), FP32 or FP16
+ *   accept_uniforms fp32 [batch, drafts], sample_uniforms fp32 [batch]: random
+ *            numbers in [0, 1)
+ *   tokens   int64 [batch, drafts + 1]: the accepted drafts, the next token
+ *            (-1 if its row has no weight), then -1
+ *   counts   int32 [batch]: accepted drafts + 1
+ * Draft i is accepted while accept_uniforms[b][i] * q_i(x_i) < p_i(x_i) (the
+ * product rounded to FP32). The next token is drawn from max(p - q, 0) of the
+ * first rejected position (without draft_probs: p without x), from p after the
+ * last draft when none was rejected; if the difference leaves nothing, from p.
+ * Drawing: the first token whose running sum of floor(min(w, 1) * 2^40) is
+ * above floor(u * total); NaN and negative weights count as 0. The sums are
+ * 64-bit integers, so the result is exact. vocab <= 2^22. A drafted token
+ * outside the vocabulary is rejected and sets a device error bit. No workspace;
+ * capturable.
+ */
+PDB_API int pdb_verify_drafts(const int64_t* draft_tokens, const void* target_probs,
+                              const void* draft_probs, const float* accept_uniforms,
+                              const float* sample_uniforms, const int32_t* draft_lengths,
+                              int64_t* tokens, int32_t* counts, int64_t batch, int64_t drafts,
+                              int64_t vocab, int dtype, void* stream);
+
+/*
+ * Eviction from a paged cache by accumulated attention weight. No reference
+ * counterpart (its cache keeps every token until the request ends).
+ * Per sequence and kv head, min(lengths[b], budget) tokens stay: the last
+ * `recent` and, of the others, those of highest score (NaN lowest; equal
+ * scores: lowest index). In their order, their K and V rows are copied to
+ * cells 0, 1, ... of the pages new_tables[b] of the same pools, and their scores.
+ *   scores   fp32 [batch, kv_heads, scores_width] by own token, e.g. as
+ *            pdb_shared_prefix_attention accumulates them
+ *   tables int32 [batch, table_width], lengths int32 [batch]
+ *   new_tables int32 [batch, new_table_width]: pages that hold the budget;
+ *            they must be in no table that is still read (reserve them, evict
+ *            every layer, then release the old ones)
+ *   kept     int32 [batch, kv_heads, budget]: indices of the kept tokens,
+ *            ascending, then -1
+ *   new_lengths int32 [batch]; new_scores fp32 like scores, 0 past the kept
+ * Lengths out of range are clamped, pages out of range skipped; both set
+ * device error bits. No workspace; capturable.
+ */
+PDB_API int pdb_evict_tokens(void* k_pool, void* v_pool, const float* scores,
+                             int64_t scores_width, const int32_t* tables, const int32_t* lengths,
+                             const int32_t* new_tables, int32_t* kept, int32_t* new_lengths,
+                             float* new_scores, int64_t batch, int64_t head_dim,
+                             int64_t num_blocks, int64_t block_size, int64_t kv_heads,
+                             int64_t table_width, int64_t new_table_width, int64_t budget,
+                             int64_t recent, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
