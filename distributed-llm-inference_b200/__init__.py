@@ -32,7 +32,7 @@ from ._lib import PREFILL_AUTO, PREFILL_MMA, PREFILL_TCGEN05  # noqa: F401
 from .ops import (decode_attention, decode_attention_supported,  # noqa: F401
                   fast_grid_size, paged_attention, prefill_attention, read_device_errors,
                   rope_kv_write, rope_kv_write_decode)
-from ._lib import PREFIX_AUTO, PREFIX_SIMT  # noqa: F401
+from ._lib import PREFIX_AUTO, PREFIX_MMA, PREFIX_SIMT, PREFIX_TCGEN05  # noqa: F401
 from .serving_ops import evict_tokens, shared_prefix_attention, verify_drafts  # noqa: F401
 from .paged_kv import DevicePagedKV  # noqa: F401
 from .llama_runner import PagedLlama  # noqa: F401
@@ -46,5 +46,6 @@ __all__ = [
     "cuda_paged_attention", "install", "uninstall",
     "read_device_errors", "fast_grid_size", "load_library",
     "IMPL_AUTO", "IMPL_FAST", "IMPL_GENERIC", "IMPL_SIMT", "IMPL_MMA", "IMPL_TMA_STATIC",
+    "PREFIX_AUTO", "PREFIX_SIMT", "PREFIX_MMA", "PREFIX_TCGEN05",
     "PREFILL_AUTO", "PREFILL_TCGEN05", "PREFILL_MMA",
 ]

@@ -3,7 +3,11 @@
 // layout and launches. Included by paged_decode.cu, whose helpers it uses.
 #pragma once
 
+#include <algorithm>
+
 #include "shared_prefix.cuh"
+#include "shared_prefix_mma.cuh"
+#include "shared_prefix_tc.cuh"
 #include "verify.cuh"
 #include "evict.cuh"
 
@@ -14,47 +18,109 @@ int page_shift(int64_t bs) {
 }
 
 // ---- shared-prefix attention -------------------------------------------------
-struct PrefixPlan {
-  int prefix_slots, prefix_chunk, own_slots, own_chunk;
-  size_t ml_off, o_off, lse_off, logits_off, total;
-};
+// The kernel of one key set: the FP32 pipes, warp-level tensor cores, tcgen05.
+enum SpanKernel { kSpanNone = 0, kSpanSimt, kSpanMma, kSpanTc };
 
-// Splits `keys` into ranges of a multiple of 64 keys, no shorter than `least`,
-// so that `tiles` CTAs per range reach `want` CTAs where the keys allow it.
-void split_keys(int64_t keys, int64_t tiles, int64_t want, int64_t least, int* slots, int* chunk) {
-  if (keys <= 0) {
-    *slots = 0;
-    *chunk = 64;
-    return;
-  }
-  int64_t s = (want + tiles - 1) / tiles;
-  const int64_t most = (keys + least - 1) / least;
-  if (s > most) s = most;
-  if (s < 1) s = 1;
-  int64_t c = (keys + s - 1) / s;
-  c = (c + 63) / 64 * 64;
-  *chunk = (int)c;
-  *slots = (int)((keys + c - 1) / c);
-}
+struct PrefixPlan {
+  int prefix_kernel, own_kernel;
+  int prefix_nt, own_nt;  // kSpanMma: 8-row tiles per segment
+  pdb::PartSet prefix, own;
+  size_t prefix_ml, prefix_o, own_ml, own_o, start_off, lse_off, logits_off, total;
+};
 
 constexpr int kPrefixSimtRows = 32;
 int simt_rows(int64_t rows) { return rows <= 8 ? 8 : kPrefixSimtRows; }
 
-PrefixPlan prefix_plan(int64_t B, int64_t T, int64_t H, int64_t KVH, int64_t D, int64_t P,
-                       int64_t max_length, bool scored) {
+// Key ranges for the FP32 kernel: a multiple of 64 keys, no shorter than
+// `least`, so that `tiles` CTAs per range reach `want` CTAs where the keys allow.
+void split_keys(int64_t keys, int64_t tiles, int64_t want, int64_t least, pdb::PartSet* s) {
+  int64_t n = (want + tiles - 1) / tiles;
+  const int64_t most = (keys + least - 1) / least;
+  if (n > most) n = most;
+  if (n < 1) n = 1;
+  int64_t c = (keys + n - 1) / n;
+  c = (c + 63) / 64 * 64;
+  s->kind = pdb::kPartSlots;
+  s->chunk = (int)c;
+  s->slots = (int)((keys + c - 1) / c);
+}
+// Rows per segment of the mma.sync kernel, in tiles of 8: the K and V tiles are
+// read once per segment, so as many rows as there are, up to 32 (registers).
+int span_nt(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+
+constexpr int kSpanCtasPerSm = 2;
+// From this many rows on, a prefix goes to the tcgen05 kernel (128-row tiles).
+constexpr int64_t kTcRows = 64;
+
+PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, int64_t D, int64_t P,
+                       int64_t max_length, bool scored, bool tensor_cores, int impl) {
   PrefixPlan pl{};
-  const int64_t TG = T * (H / KVH), rows = B * T * H;
-  const int64_t pt = (B * TG + simt_rows(B * TG) - 1) / simt_rows(B * TG);
-  const int64_t ot = (TG + simt_rows(TG) - 1) / simt_rows(TG);
-  split_keys(P, pt * KVH, 4 * 148, 64, &pl.prefix_slots, &pl.prefix_chunk);
-  split_keys(max_length, ot * B * KVH, 8 * 148, 128, &pl.own_slots, &pl.own_chunk);
-  const size_t slots = (size_t)pl.prefix_slots + pl.own_slots;
-  pl.ml_off = 0;
-  pl.o_off = align256(slots * rows * sizeof(float2));
-  pl.lse_off = pl.o_off + align256(slots * rows * D * sizeof(float));
-  pl.logits_off = pl.lse_off + (scored ? align256((size_t)rows * sizeof(float)) : 0);
-  pl.total = pl.logits_off +
-             (scored ? align256((size_t)rows * (size_t)max_length * sizeof(float)) : 0);
+  const int64_t G = H / KVH, TG = T * G, rows = B * T * H, all = B * TG;
+  pl.prefix_kernel = P <= 0 ? kSpanNone : kSpanSimt;
+  pl.own_kernel = max_length <= 0 ? kSpanNone : kSpanSimt;
+  if (tensor_cores && impl != PDB_PREFIX_SIMT) {
+    if (pl.own_kernel) pl.own_kernel = kSpanMma;
+    if (pl.prefix_kernel) {
+      const bool tc = G <= 128 && (impl == PDB_PREFIX_TCGEN05 ||
+                                   (impl == PDB_PREFIX_AUTO && all >= kTcRows));
+      pl.prefix_kernel = tc ? kSpanTc : kSpanMma;
+    }
+  }
+  size_t prefix_parts = 0, own_parts = 0;
+  if (pl.prefix_kernel == kSpanSimt) {
+    split_keys(P, (all + simt_rows(all) - 1) / simt_rows(all) * KVH, 4 * (int64_t)sms, 64, &pl.prefix);
+    prefix_parts = (size_t)pl.prefix.slots * rows;
+  } else if (pl.prefix_kernel == kSpanMma) {
+    pl.prefix_nt = span_nt(all);
+    pdb::PartSet& s = pl.prefix;
+    s.kind = pdb::kPartUnits;
+    s.R = 8 * pl.prefix_nt;
+    s.segments = (int)((all + s.R - 1) / s.R);
+    s.overhead = pdb::kSpanOverhead;
+    s.seg_units = (int)((P + 63) / 64) + s.overhead;
+    const int64_t units = KVH * s.segments * (int64_t)s.seg_units;
+    s.grid = (int)std::min<int64_t>(kSpanCtasPerSm * (int64_t)sms, units);
+    prefix_parts = (size_t)(KVH * s.segments + s.grid) * s.R;
+  } else if (pl.prefix_kernel == kSpanTc) {
+    pdb::PartSet& s = pl.prefix;
+    s.kind = pdb::kPartUnits;
+    s.R = 256;
+    s.half = (int)(128 / G);
+    s.segments = (int)((B * T + 2 * s.half - 1) / (2 * s.half));
+    s.seg_units = (int)((P + 127) / 128);
+    const int64_t units = KVH * s.segments * (int64_t)s.seg_units;
+    s.grid = (int)std::min<int64_t>(sms, units);
+    prefix_parts = (size_t)(KVH * s.segments + s.grid) * s.R;
+  }
+  if (pl.own_kernel == kSpanSimt) {
+    split_keys(max_length, (TG + simt_rows(TG) - 1) / simt_rows(TG) * B * KVH, 8 * (int64_t)sms, 128,
+               &pl.own);
+    own_parts = (size_t)pl.own.slots * rows;
+  } else if (pl.own_kernel == kSpanMma) {
+    pl.own_nt = span_nt(TG);
+    pdb::PartSet& s = pl.own;
+    s.kind = pdb::kPartUnits;
+    s.R = 8 * pl.own_nt;
+    s.segments = (int)((TG + s.R - 1) / s.R);
+    s.overhead = pdb::kSpanOverhead;
+    const int64_t units = B * KVH * s.segments * ((max_length + 63) / 64 + s.overhead);
+    s.grid = (int)std::min<int64_t>(kSpanCtasPerSm * (int64_t)sms, units);
+    own_parts = (size_t)(B * KVH * s.segments + s.grid) * s.R;
+  }
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  pl.prefix_ml = take(prefix_parts * sizeof(float2));
+  pl.prefix_o = take(prefix_parts * D * sizeof(float));
+  pl.own_ml = take(own_parts * sizeof(float2));
+  pl.own_o = take(own_parts * D * sizeof(float));
+  pl.start_off = take(pl.own_kernel == kSpanMma ? (size_t)(B + 1) * sizeof(int64_t) : 0);
+  pl.lse_off = take(scored ? (size_t)rows * sizeof(float) : 0);
+  pl.logits_off = take(scored ? (size_t)rows * (size_t)max_length * sizeof(float) : 0);
+  pl.total = at;
   return pl;
 }
 
@@ -67,8 +133,8 @@ cudaError_t launch_prefix_simt(int dev, const pdb::PrefixParams& p, bool prefix,
   const int64_t TG = (int64_t)p.T * p.G;
   const int prefix_tiles = prefix ? (int)((p.B * TG + RT - 1) / RT) : 0;
   const int own_tiles = prefix ? 0 : (int)((TG + RT - 1) / RT);
-  const int64_t gx = prefix ? (int64_t)prefix_tiles * p.prefix_slots
-                            : (int64_t)p.B * own_tiles * p.own_slots;
+  const int64_t gx = prefix ? (int64_t)prefix_tiles * p.prefix.slots
+                            : (int64_t)p.B * own_tiles * p.own.slots;
   return launch_pdl(fn, dim3((unsigned)gx, (unsigned)p.KVH), dim3(C::NT), C::SMEM, st, p,
                     prefix_tiles, own_tiles);
 }
@@ -92,6 +158,83 @@ cudaError_t launch_spans_simt(int dev, int dtype, const pdb::PrefixParams& p, bo
   return launch_prefix_simt_rows<float, 256>(dev, p, prefix, st);
 }
 
+template <int D, int NT>
+cudaError_t launch_span_mma(int dev, const pdb::PrefixParams& p, const pdb::SpanSet& ss, int grid,
+                            cudaStream_t st, const CUtensorMap& kmap, const CUtensorMap& vmap) {
+  using C = pdb::SpanMma<D, NT, D == 64 ? 2 : 1, (D == 128 && NT == 4) ? 2 : 3, true>;
+  auto* fn = &pdb::prefix_span_kernel<C>;
+  if (ctas_per_sm(dev, reinterpret_cast<const void*>(fn), C::SMEM, C::THREADS) <= 0)
+    return cudaErrorInvalidConfiguration;
+  return launch_pdl(fn, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, st, p, ss, kmap, vmap);
+}
+cudaError_t launch_spans_mma(int dev, const pdb::PrefixParams& p, const PrefixPlan& pl, bool prefix,
+                             cudaStream_t st, const CUtensorMap& kmap, const CUtensorMap& vmap) {
+  pdb::SpanSet ss{};
+  ss.part = prefix ? p.prefix : p.own;
+  ss.own = prefix ? 0 : 1;
+  ss.tables = prefix ? p.prefix_table : p.tables;
+  ss.width = prefix ? (p.prefix_length + p.block_size - 1) / p.block_size : p.table_width;
+  ss.nseq = prefix ? 1 : p.B;
+  ss.tokens = prefix ? p.B * p.T : p.T;
+  ss.rows = ss.tokens * p.G;
+  ss.start = p.own_start;
+  const int nt = prefix ? pl.prefix_nt : pl.own_nt, grid = ss.part.grid;
+  if (p.D == 64) {
+    if (nt == 1) return launch_span_mma<64, 1>(dev, p, ss, grid, st, kmap, vmap);
+    if (nt == 2) return launch_span_mma<64, 2>(dev, p, ss, grid, st, kmap, vmap);
+    return launch_span_mma<64, 4>(dev, p, ss, grid, st, kmap, vmap);
+  }
+  if (nt == 1) return launch_span_mma<128, 1>(dev, p, ss, grid, st, kmap, vmap);
+  if (nt == 2) return launch_span_mma<128, 2>(dev, p, ss, grid, st, kmap, vmap);
+  return launch_span_mma<128, 4>(dev, p, ss, grid, st, kmap, vmap);
+}
+
+// Query tiles of the tcgen05 kernel: box {64 columns, G heads, `tokens` tokens}.
+bool encode_group_map(CUtensorMap* m, const void* q, int64_t R, int64_t heads, int64_t D, int G,
+                      int tokens) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)R};
+  const cuuint64_t strides[2] = {(cuuint64_t)(D * 2), (cuuint64_t)(heads * D * 2)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)tokens};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+template <int D>
+cudaError_t launch_prefix_tc(int dev, const pdb::PrefixParams& p, cudaStream_t st,
+                             const CUtensorMap& kmap, const CUtensorMap& vmap) {
+  using C = pdb::PrefixTc<D>;
+  auto* fn = &pdb::prefix_tc_kernel<D>;
+  if (ctas_per_sm(dev, reinterpret_cast<const void*>(fn), C::SMEM, C::THREADS) <= 0)
+    return cudaErrorInvalidConfiguration;
+  pdb::PrefixTcParams t{};
+  t.table = p.prefix_table;
+  t.ml = p.prefix.ml;
+  t.o = p.prefix.o;
+  t.num_blocks = p.num_blocks;
+  t.tokens = p.B * p.T;
+  t.H = p.H; t.KVH = p.KVH; t.G = p.G;
+  t.per_tile = p.prefix.half;
+  t.pairs = p.prefix.segments;
+  t.key_tiles = p.prefix.seg_units;
+  t.prefix_length = p.prefix_length;
+  t.block_size = p.block_size; t.bs_shift = p.bs_shift;
+  t.scale_log2 = p.scale_log2;
+  CUtensorMap qmap;
+  if (!encode_group_map(&qmap, p.q, t.tokens, p.H, D, p.G, t.per_tile)) return cudaErrorInvalidValue;
+  return launch_pdl(fn, dim3((unsigned)p.prefix.grid), dim3(C::THREADS), C::SMEM, st, t, qmap, kmap,
+                    vmap);
+}
+
+// Whether the tensor-core kernels take this shape (pointers aside).
+bool prefix_tensor_cores(int64_t D, int64_t num_blocks, int64_t block_size, int dtype) {
+  return dtype == PDB_DTYPE_FLOAT16 && (D == 64 || D == 128) &&
+         block_size % pdb::kUnitTokens == 0 && num_blocks * block_size <= INT32_MAX &&
+         tensor_map_encoder() != nullptr;
+}
+
 // Sizes that every kernel's 32-bit indices can hold.
 bool prefix_sizes_ok(int64_t B, int64_t T, int64_t H, int64_t D, int64_t KVH, int64_t P,
                      int64_t max_length) {
@@ -108,14 +251,26 @@ size_t pdb_shared_prefix_attention_workspace_size(int64_t batch, int64_t tokens,
                                                   int64_t kv_heads, int64_t head_dim,
                                                   int64_t prefix_length, int64_t max_length,
                                                   int dtype, int with_scores) {
-  (void)dtype;
   if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
       heads % kv_heads || prefix_length < 0 || max_length < 0 ||
       !prefix_sizes_ok(batch, tokens, heads, head_dim, kv_heads, prefix_length, max_length))
     return 0;
-  return prefix_plan(batch, tokens, heads, kv_heads, head_dim, prefix_length, max_length,
-                     with_scores != 0)
-      .total;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  // the pool is not known here: cover every kernel that a call may select
+  const int sms = sm_count(dev);
+  size_t need = 0;
+  const int impls[4] = {PDB_PREFIX_AUTO, PDB_PREFIX_SIMT, PDB_PREFIX_MMA, PDB_PREFIX_TCGEN05};
+  for (const int impl : impls) {
+    const size_t n =
+        prefix_plan(sms, batch, tokens, heads, kv_heads, head_dim, prefix_length, max_length,
+                    with_scores != 0, prefix_tensor_cores(head_dim, 1, 16, dtype), impl).total;
+    if (n > need) need = n;
+  }
+  return need;
 }
 
 int pdb_shared_prefix_attention_impl(
@@ -148,29 +303,38 @@ int pdb_shared_prefix_attention_impl(
   if (scores && scores_width < max_length)
     return fail(PDB_ERR_INVALID_ARGUMENT, "scores must hold max_length tokens");
   if (scores && scores_width > INT32_MAX) return fail(PDB_ERR_INVALID_ARGUMENT, "shape too large");
-  if (impl < PDB_PREFIX_AUTO || impl > PDB_PREFIX_SIMT)
+  if (impl < PDB_PREFIX_AUTO || impl > PDB_PREFIX_TCGEN05)
     return fail(PDB_ERR_INVALID_ARGUMENT, "unknown kernel selection");
   if (!q || !k_pool || !v_pool || !lengths || !out || (prefix_length > 0 && !prefix_table) ||
       (max_length > 0 && !tables))
     return fail(PDB_ERR_INVALID_ARGUMENT, "null tensor pointer");
-  const PrefixPlan pl = prefix_plan(batch, tokens, heads, kv_heads, head_dim, prefix_length,
-                                    max_length, scores != nullptr);
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  const bool tensor_cores = prefix_tensor_cores(head_dim, num_blocks, block_size, dtype) &&
+                            aligned16(q) && aligned16(k_pool) && aligned16(v_pool);
+  if (impl > PDB_PREFIX_SIMT && !tensor_cores)
+    return fail(PDB_ERR_INVALID_ARGUMENT, "tensor-core kernels do not support this shape/alignment");
+  const PrefixPlan pl = prefix_plan(sm_count(dev), batch, tokens, heads, kv_heads, head_dim,
+                                    prefix_length, max_length, scores != nullptr, tensor_cores, impl);
   if (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return fail(PDB_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   if (pl.total && (!workspace || workspace_bytes < pl.total))
     return fail(PDB_ERR_WORKSPACE,
                 "workspace too small: need " + std::to_string(pl.total) + " bytes");
-  int dev = 0;
-  int rc = current_device(&dev);
-  if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   unsigned char* wb = static_cast<unsigned char*>(workspace);
   pdb::PrefixParams p{};
   p.q = q; p.k_pool = k_pool; p.v_pool = v_pool;
   p.prefix_table = prefix_table; p.tables = tables; p.lengths = lengths; p.counts = counts;
   p.out = out;
-  p.ml = reinterpret_cast<float2*>(wb + pl.ml_off);
-  p.o = reinterpret_cast<float*>(wb + pl.o_off);
+  p.prefix = pl.prefix;
+  p.prefix.ml = reinterpret_cast<float2*>(wb + pl.prefix_ml);
+  p.prefix.o = reinterpret_cast<float*>(wb + pl.prefix_o);
+  p.own = pl.own;
+  p.own.ml = reinterpret_cast<float2*>(wb + pl.own_ml);
+  p.own.o = reinterpret_cast<float*>(wb + pl.own_o);
+  p.own_start = reinterpret_cast<int64_t*>(wb + pl.start_off);
   if (scores) {
     p.lse = reinterpret_cast<float*>(wb + pl.lse_off);
     p.logits = reinterpret_cast<float*>(wb + pl.logits_off);
@@ -183,17 +347,36 @@ int pdb_shared_prefix_attention_impl(
   p.block_size = (int)block_size; p.bs_shift = page_shift(block_size);
   p.table_width = (int)table_width;
   p.prefix_length = (int)prefix_length; p.max_length = (int)max_length;
-  p.prefix_slots = pl.prefix_slots; p.prefix_chunk = pl.prefix_chunk;
-  p.own_slots = pl.own_slots; p.own_chunk = pl.own_chunk;
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
+  CUtensorMap kmap, vmap;
+  if (tensor_cores && !(encode_pool_map(&kmap, k_pool, num_blocks, block_size, kv_heads, head_dim) &&
+                        encode_pool_map(&vmap, v_pool, num_blocks, block_size, kv_heads, head_dim)))
+    return fail(PDB_ERR_CUDA, "cuTensorMapEncodeTiled failed for the KV pools");
   cudaError_t e = cudaSuccess;
-  if (p.prefix_slots) e = launch_spans_simt(dev, dtype, p, true, st);
-  if (e == cudaSuccess && p.own_slots) e = launch_spans_simt(dev, dtype, p, false, st);
+  if (pl.prefix_kernel == kSpanTc)
+    e = head_dim == 64 ? launch_prefix_tc<64>(dev, p, st, kmap, vmap)
+                       : launch_prefix_tc<128>(dev, p, st, kmap, vmap);
+  else if (pl.prefix_kernel == kSpanMma)
+    e = launch_spans_mma(dev, p, pl, true, st, kmap, vmap);
+  else if (pl.prefix_kernel == kSpanSimt)
+    e = launch_spans_simt(dev, dtype, p, true, st);
+  if (e == cudaSuccess && pl.own_kernel == kSpanMma)
+    e = launch_spans_mma(dev, p, pl, false, st, kmap, vmap);
+  else if (e == cudaSuccess && pl.own_kernel == kSpanSimt)
+    e = launch_spans_simt(dev, dtype, p, false, st);
   if (e == cudaSuccess) {
-    const dim3 grid((unsigned)((p.rows + 7) / 8));
-    e = dtype == PDB_DTYPE_FLOAT16
-            ? launch_pdl(pdb::prefix_join_kernel<__half>, grid, dim3(256), 0, st, p)
-            : launch_pdl(pdb::prefix_join_kernel<float>, grid, dim3(256), 0, st, p);
+    auto join = [&](auto* fn, int lanes) {
+      return launch_pdl(fn, dim3((unsigned)((p.rows * lanes + 255) / 256)), dim3(256), 0, st, p);
+    };
+    const bool vec = head_dim % 4 == 0 && head_dim <= 128;
+    if (dtype == PDB_DTYPE_FLOAT16)
+      e = !vec             ? join(pdb::prefix_join_kernel<__half, 32, false>, 32)
+          : head_dim <= 64 ? join(pdb::prefix_join_kernel<__half, 16, true>, 16)
+                           : join(pdb::prefix_join_kernel<__half, 32, true>, 32);
+    else
+      e = !vec             ? join(pdb::prefix_join_kernel<float, 32, false>, 32)
+          : head_dim <= 64 ? join(pdb::prefix_join_kernel<float, 16, true>, 16)
+                           : join(pdb::prefix_join_kernel<float, 32, true>, 32);
   }
   if (e == cudaSuccess && scores && scores_width > 0)
     e = launch_pdl(pdb::prefix_scores_kernel,

@@ -12,17 +12,44 @@
 // sequence) and a sequence's own tokens are another for its T G rows.
 //
 // Rows of a kv head are numbered r = (b T + t) G + g; the rows of sequence b
-// are [b T G, (b + 1) T G). A "span" is (rows, kv head, key range): its
-// partial goes to slot `slot` of the workspace, at the global row
-// (b T + t) H + h, the row order of q and out:
-//   ml [slots][rows] float2 (m, l), o [slots][rows][D] fp32.
-// Slots 0 .. prefix_slots - 1 are the prefix's key ranges, the others the
-// chunks of own tokens. prefix_join_kernel joins the slots that a row has.
+// are [b T G, (b + 1) T G). A partial is (m, l) and O of some rows over a key
+// range, in FP32: ml [..] float2, o [..][D]. The prefix's partials and those of
+// own tokens are two sets (PartSet), each written by one of these kernels:
+//   * the FP32 kernel here: fixed key ranges ("slots") of every row,
+//     part index = slot * rows + global row (b T + t) H + h;
+//   * the tensor-core kernels: work in units (64- or 128-key tiles of a segment
+//     of rows), cut into one contiguous range per CTA; CTA c's piece of segment
+//     s is stored as piece s + c (distinct for distinct pieces, as each step to
+//     the next piece raises s, c or both), part index = piece * R + row of the
+//     segment. The pieces of a segment are those of consecutive CTAs.
+// Either way a row's partials are evenly spaced: prefix_join_kernel joins them.
 #pragma once
 
 #include "attention.cuh"
 
 namespace pdb {
+
+// CTAs that share `units`: each has at least one, so that the pieces of a
+// segment are those of consecutive CTAs.
+__host__ __device__ __forceinline__ int64_t unit_ctas(int64_t units, int64_t grid) {
+  return units < grid ? units : grid;
+}
+
+enum : int { kPartNone = 0, kPartSlots = 1, kPartUnits = 2 };
+
+struct PartSet {
+  float2* ml;
+  float* o;
+  int kind;
+  int slots, chunk;   // kPartSlots: key ranges [i * chunk, (i + 1) * chunk)
+  int R;              // kPartUnits: rows of a segment
+  int tokens;         //   tokens (all G heads of a kv head) that a segment's rows hold
+  int half;           //   tokens of its first R / 2 rows (two query tiles), or 0: rows are dense
+  int segments;       //   segments per (sequence,) kv head
+  int grid;           //   CTAs that share the units
+  int seg_units;      //   units of a segment of the prefix
+  int overhead;       //   of them at its start that hold no keys
+};
 
 struct PrefixParams {
   const void* q;                // [B, T, H, D]
@@ -33,18 +60,16 @@ struct PrefixParams {
   const int32_t* lengths;       // [B]
   const int32_t* counts;        // [B] or NULL (all T)
   void* out;                    // [B, T, H, D]
-  float2* ml;                   // [slots][rows]
-  float* o;                     // [slots][rows][D]
+  PartSet prefix, own;          // partials
+  int64_t* own_start;           // [B + 1] first unit of each sequence (tensor-core kernel)
   float* lse;                   // [rows] base-2 log of the softmax's denominator (scores only)
-  float* logits;                // [B, KVH, T G, logits_width] base-2 logits of own tokens, or NULL
+  float* logits;                // [B, KVH, logits_width, T G] base-2 logits of own tokens, or NULL
   const float* scores;          // [B, KVH, scores_width]
   float* scores_out;
   int64_t num_blocks, rows, logits_width, scores_width;
   int B, T, H, KVH, G, D;
   int block_size, bs_shift, table_width;
   int prefix_length, max_length;
-  int prefix_slots, prefix_chunk;  // key ranges of the prefix: [i * chunk, (i + 1) * chunk)
-  int own_slots, own_chunk;        // the same for own tokens
   float scale_log2;
 };
 
@@ -114,27 +139,27 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
   int x = blockIdx.x, b = -1, slot, k0, k1, n = 0, count = 0, width;
   int64_t r0, rend;  // rows of this tile in the kv head's numbering
   const int32_t* table;
-  const int npre = prefix_tiles * p.prefix_slots;
+  const int npre = prefix_tiles * p.prefix.slots;
+  const PartSet& set = x < npre ? p.prefix : p.own;
   if (x < npre) {
-    slot = x % p.prefix_slots;
-    r0 = (int64_t)(x / p.prefix_slots) * RT;
+    slot = x % set.slots;
+    r0 = (int64_t)(x / set.slots) * RT;
     rend = (int64_t)p.B * p.T * G;
-    k0 = slot * p.prefix_chunk;
-    k1 = k0 + p.prefix_chunk < p.prefix_length ? k0 + p.prefix_chunk : p.prefix_length;
+    k0 = slot * set.chunk;
+    k1 = k0 + set.chunk < p.prefix_length ? k0 + set.chunk : p.prefix_length;
     table = p.prefix_table;
     width = (p.prefix_length + p.block_size - 1) / p.block_size;
   } else {
     x -= npre;
-    const int c = x % p.own_slots;
-    x /= p.own_slots;
+    slot = x % set.slots;
+    x /= set.slots;
     const int tile = x % own_tiles;
     b = x / own_tiles;
     prefix_sequence(p, b, n, count);
-    slot = p.prefix_slots + c;
     r0 = (int64_t)b * p.T * G + (int64_t)tile * RT;
     rend = (int64_t)(b + 1) * p.T * G;
-    k0 = c * p.own_chunk;
-    k1 = k0 + p.own_chunk < n ? k0 + p.own_chunk : n;
+    k0 = slot * set.chunk;
+    k1 = k0 + set.chunk < n ? k0 + set.chunk : n;
     table = p.tables + (int64_t)b * p.table_width;
     width = p.table_width;
     if (k0 >= k1) return;
@@ -158,8 +183,8 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
 #pragma unroll
   for (int i = 0; i < OD; ++i) acc[i] = 0.f;
   float* logits = (p.logits && b >= 0 && row < rend)
-                      ? p.logits + (((int64_t)b * p.KVH + h) * p.T * G + (row - (int64_t)b * p.T * G)) *
-                                       p.logits_width
+                      ? p.logits + ((int64_t)b * p.KVH + h) * p.logits_width * p.T * G +
+                            (row - (int64_t)b * p.T * G)
                       : nullptr;
 
   for (int t0 = k0; t0 < k1; t0 += KT) {
@@ -192,7 +217,7 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
     for (int i = 0; i < SK; ++i) {
       const int key = t0 + part + i * TPR;
       s[i] = (key < limit && key < k1) ? s[i] * p.scale_log2 : -INFINITY;
-      if (logits && key < limit && key < k1) logits[key] = s[i];
+      if (logits && key < limit && key < k1) logits[(int64_t)key * p.T * G] = s[i];
       mt = fmaxf(mt, s[i]);
     }
 #pragma unroll
@@ -220,50 +245,125 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
   for (int o = 1; o < TPR; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   if (row >= rend) return;
   const int64_t at = (int64_t)slot * p.rows + (row / G) * p.H + (int64_t)h * G + row % G;
-  if (part == 0) p.ml[at] = make_float2(m, l);
+  if (part == 0) set.ml[at] = make_float2(m, l);
 #pragma unroll
   for (int i = 0; i < OD; ++i)
-    if (part + i * TPR < D) p.o[at * D + part + i * TPR] = acc[i];
+    if (part + i * TPR < D) set.o[at * D + part + i * TPR] = acc[i];
 }
 
 // ---- join of the partials -----------------------------------------------------
-// One warp per row (b, t, h). Slots are visited in order, so the sum does not
-// depend on which span finished first.
-template <typename T>
+// A row's partials in one set: part indices at, at + step, .. (count of them).
+struct PartRange {
+  int64_t at, step;
+  int count;
+};
+__device__ __forceinline__ PartRange prefix_parts(const PartSet& s, int64_t rows, int64_t row,
+                                                  int used_slots, int64_t seg, int64_t first_unit,
+                                                  int64_t last_unit, int64_t units, int lr) {
+  if (s.kind == kPartSlots) return PartRange{row, rows, used_slots};
+  const int64_t ctas = unit_ctas(units, s.grid);
+  const int64_t c0 = part_owner(first_unit, units, ctas), c1 = part_owner(last_unit, units, ctas);
+  return PartRange{(seg + c0) * s.R + lr, s.R, (int)(c1 - c0) + 1};
+}
+// Row of token `t` (of those that share segments) and head g of the group: its
+// segment among them and its row there.
+__device__ __forceinline__ int prefix_segment(const PartSet& s, int64_t t, int g, int G, int* lr) {
+  if (s.half) {  // two query tiles of R / 2 rows, each with a remainder of unused rows
+    const int seg = (int)(t / (2 * s.half)), in = (int)(t - (int64_t)seg * 2 * s.half);
+    *lr = (in / s.half) * (s.R / 2) + (in % s.half) * G + g;
+    return seg;
+  }
+  const int64_t r = t * G + g;
+  *lr = (int)(r % s.R);
+  return (int)(r / s.R);
+}
+
+// VEC: D % 4 == 0 and D <= 128, four dims per lane, LPR lanes per row (D / 4
+// rounded up to 16 or 32); else up to 8 strided dims per lane, 32 lanes. Partials
+// are visited in order, so the sum does not depend on which CTA finished first.
+template <typename T, int LPR, bool VEC>
 __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) {
   grid_dependency_wait();
   launch_dependents();
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, D = p.D;
-  if (row >= p.rows) return;
+  constexpr int NV = VEC ? 4 : 8;
+  int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  const int lane = threadIdx.x % LPR, D = p.D;
+  const bool real = row < p.rows;  // the others follow along for the shuffles
+  if (!real) row = p.rows - 1;
   const int64_t bt = row / p.H;
-  const int b = (int)(bt / p.T);
+  const int b = (int)(bt / p.T), t = (int)(bt % p.T), hq = (int)(row % p.H), h = hq / p.G,
+            g = hq % p.G;
   int n, count;
   prefix_sequence(p, b, n, count);
-  const int limit = prefix_limit(n, count, (int)(bt % p.T));
-  const int own = limit > 0 ? (limit + p.own_chunk - 1) / p.own_chunk : 0;
-  const int used = limit < 0 ? 0 : p.prefix_slots + own;
-  float m = -INFINITY;
-  for (int s = lane; s < used; s += 32) m = fmaxf(m, p.ml[(int64_t)s * p.rows + row].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float l = 0.f, acc[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-  for (int s = 0; s < used; ++s) {
-    const float2 v = p.ml[(int64_t)s * p.rows + row];
-    const float w = v.x == -INFINITY ? 0.f : exp2f(v.x - m);
-    l = fmaf(w, v.y, l);
-    const float* src = p.o + ((int64_t)s * p.rows + row) * D;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < D) acc[i] = fmaf(w, src[lane + 32 * i], acc[i]);
+  const int limit = prefix_limit(n, count, t);
+  PartRange part[2] = {{0, 0, 0}, {0, 0, 0}};
+  if (limit >= 0 && p.prefix.kind) {
+    int lr = 0;
+    const int64_t seg = p.prefix.kind == kPartUnits
+                            ? (int64_t)h * p.prefix.segments + prefix_segment(p.prefix, bt, g, p.G, &lr)
+                            : 0;
+    const int64_t u = seg * p.prefix.seg_units;
+    part[0] = prefix_parts(p.prefix, p.rows, row, p.prefix.slots, seg, u + p.prefix.overhead,
+                           u + p.prefix.seg_units - 1,
+                           (int64_t)p.KVH * p.prefix.segments * p.prefix.seg_units, lr);
   }
+  if (limit > 0 && p.own.kind) {
+    int lr = 0;
+    int64_t in = 0, first = 0, last = 0, total = 0;
+    if (p.own.kind == kPartUnits) {
+      in = (int64_t)h * p.own.segments + prefix_segment(p.own, t, g, p.G, &lr);
+      const int keys = (n + 63) / 64;
+      first = p.own_start[b] + in * (keys + p.own.overhead) + p.own.overhead;
+      last = first + keys - 1;
+      total = p.own_start[p.B];
+    }
+    part[1] = prefix_parts(p.own, p.rows, row, p.own.kind == kPartSlots
+                                                   ? (limit + p.own.chunk - 1) / p.own.chunk : 0,
+                           (int64_t)b * p.KVH * p.own.segments + in, first, last, total, lr);
+  }
+  const float2* ml[2] = {p.prefix.ml, p.own.ml};
+  const float* o[2] = {p.prefix.o, p.own.o};
+  float m = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+    for (int s = lane; s < part[x].count; s += LPR)
+      m = fmaxf(m, ml[x][part[x].at + s * part[x].step].x);
+#pragma unroll
+  for (int i = LPR / 2; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+  float l = 0.f, acc[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+#pragma unroll 4
+    for (int s = 0; s < part[x].count; ++s) {
+      const int64_t at = part[x].at + s * part[x].step;
+      const float2 v = ml[x][at];
+      const float w = v.x == -INFINITY ? 0.f : exp2f(v.x - m);
+      l = fmaf(w, v.y, l);
+      if constexpr (VEC) {
+        if (4 * lane < D) {
+          const float4 f = *reinterpret_cast<const float4*>(o[x] + at * D + 4 * lane);
+          acc[0] = fmaf(w, f.x, acc[0]);
+          acc[1] = fmaf(w, f.y, acc[1]);
+          acc[2] = fmaf(w, f.z, acc[2]);
+          acc[3] = fmaf(w, f.w, acc[3]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (lane + 32 * i < D) acc[i] = fmaf(w, o[x][at * D + lane + 32 * i], acc[i]);
+      }
+    }
+  }
+  if (!real) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
   T* out = static_cast<T*>(p.out) + row * D;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < D) out[lane + 32 * i] = Elem<T>::from_f(l == 0.f ? 0.f : acc[i] * inv);
+  for (int i = 0; i < NV; ++i) {
+    const int d = VEC ? 4 * lane + i : lane + 32 * i;
+    if (d < D) out[d] = Elem<T>::from_f(l == 0.f ? 0.f : acc[i] * inv);
+  }
   if (p.lse && lane == 0) p.lse[row] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
@@ -273,21 +373,22 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
 __global__ void __launch_bounds__(256) prefix_scores_kernel(const PrefixParams p) {
   grid_dependency_wait();
   launch_dependents();
-  const int bh = blockIdx.y, b = bh / p.KVH, h = bh % p.KVH;
+  const int64_t bh = blockIdx.y;
+  const int b = (int)(bh / p.KVH), h = (int)(bh % p.KVH);
   const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (j >= p.scores_width) return;
   int n, count;
   prefix_sequence(p, b, n, count);
   float add = 0.f;
-  const float* lg = p.logits + (int64_t)bh * p.T * p.G * p.logits_width + j;
-  for (int t = 0; t < count; ++t) {
-    if (j >= prefix_limit(n, count, t)) continue;
-    for (int g = 0; g < p.G; ++g) {
-      const float lse = p.lse[((int64_t)b * p.T + t) * p.H + (int64_t)h * p.G + g];
-      add += exp2f(lg[(int64_t)(t * p.G + g) * p.logits_width] - lse);
+  if (j < n) {
+    const float* lg = p.logits + (bh * p.logits_width + j) * p.T * p.G;
+    for (int t = 0; t < count; ++t) {
+      if (j >= prefix_limit(n, count, t)) continue;
+      const float* lse = p.lse + ((int64_t)b * p.T + t) * p.H + (int64_t)h * p.G;
+      for (int g = 0; g < p.G; ++g) add += exp2f(lg[t * p.G + g] - lse[g]);
     }
   }
-  const int64_t at = (int64_t)bh * p.scores_width + j;
+  const int64_t at = bh * p.scores_width + j;
   p.scores_out[at] = p.scores[at] + add;
 }
 

@@ -23,11 +23,17 @@ from conftest import import_pkg
 pytestmark = pytest.mark.gpu
 
 TOL = {torch.float16: 1.3e-3, torch.float32: 2e-5}
-IMPLS = ["auto", "simt"]
+IMPLS = ["auto", "simt", "mma", "tcgen05"]
 
 
 def impl_of(pkg, name):
-    return {"auto": pkg.PREFIX_AUTO, "simt": pkg.PREFIX_SIMT}[name]
+    return {"auto": pkg.PREFIX_AUTO, "simt": pkg.PREFIX_SIMT, "mma": pkg.PREFIX_MMA,
+            "tcgen05": pkg.PREFIX_TCGEN05}[name]
+
+
+def covered(impl, dtype, D, bs):
+    """The tensor-core kernels take FP16, head_dim 64 and 128, whole 16-token units."""
+    return impl in ("auto", "simt") or (dtype == torch.float16 and D in (64, 128) and bs % 16 == 0)
 
 
 def pages(lengths, bs, spare, gen):
@@ -76,6 +82,10 @@ def call(pkg, d, cuda, impl="auto", **kw):
 
 
 def check(pkg, d, cuda, impl="auto"):
+    if not covered(impl, d["q"].dtype, d["q"].shape[-1], d["k"].shape[1]):
+        with pytest.raises(RuntimeError, match="tensor-core kernels do not support"):
+            call(pkg, d, cuda, impl)
+        return None
     got = call(pkg, d, cuda, impl)
     out, sc = got if "scores" in d else (got, None)
     ref, ref_sc = oracle.shared_prefix_attention(
@@ -138,6 +148,8 @@ def test_accumulated_weights(pkg, cuda, name, dtype, impl):
 @pytest.mark.parametrize("impl", IMPLS)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
 def test_sharp_and_large_logits(pkg, cuda, dtype, impl):
+    if not covered(impl, dtype, 64, 16):
+        pytest.skip("the tensor-core kernels take FP16")
     # |logit| up to ~200: the running maximum has to carry the exponentials. The
     # logits' rounding grows with them: 2^-24 * 200 * sqrt(64) is still 1e-4 of a weight.
     d = make(6, 2, 8, 2, 64, dtype, 150, [2, 9, 17, 80, 33, 64], sharp=30.0)
@@ -152,6 +164,8 @@ def test_sharp_and_large_logits(pkg, cuda, dtype, impl):
 @pytest.mark.parametrize("impl", IMPLS)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
 def test_a_later_draft_never_reaches_an_earlier_one(pkg, cuda, dtype, impl):
+    if not covered(impl, dtype, 64, 16):
+        pytest.skip("the tensor-core kernels take FP16")
     # infinities and NaN in the cells of later drafted tokens: earlier rows do not see them
     d = make(3, 4, 8, 2, 64, dtype, 30, [4, 20, 67])
     clean = call(pkg, d, cuda, impl).cpu()
@@ -163,6 +177,21 @@ def test_a_later_draft_never_reaches_an_earlier_one(pkg, cuda, dtype, impl):
         got = call(pkg, d, cuda, impl).cpu()
         assert torch.equal(got[:, :3], clean[:, :3])
         assert not torch.isfinite(got[:, 3]).any()
+
+
+@pytest.mark.parametrize("name", ["nothing to see", "ragged drafts", "long drafts", "many rows"])
+@pytest.mark.parametrize("impl", IMPLS)
+def test_workspace_contents_do_not_matter(pkg, cuda, name, impl):
+    # every partial that the join reads was written by this call: NaN bytes stay unseen
+    from conftest import import_module
+    B, T, H, KVH, D, prefix, lengths, bs, counts = ATTENTION[name]
+    d = make(B, T, H, KVH, D, torch.float16, prefix, lengths, bs, counts, scores=True)
+    first = call(pkg, dict(d), cuda, impl)
+    for key, buf in import_module("ops")._ws_cache.items():
+        if key[2] == "shared_prefix":
+            buf.fill_(0xff)
+    again = call(pkg, dict(d), cuda, impl)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
 def test_scores_in_place_and_beside(pkg, cuda):
