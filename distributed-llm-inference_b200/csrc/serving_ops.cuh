@@ -25,7 +25,7 @@ struct PrefixPlan {
   int prefix_kernel, own_kernel;
   int prefix_nt, own_nt;  // kSpanMma: 8-row tiles per segment
   pdb::PartSet prefix, own;
-  size_t prefix_ml, prefix_o, own_ml, own_o, start_off, lse_off, logits_off, total;
+  size_t prefix_ml, prefix_o, prefix_dir, own_ml, own_o, own_dir, lse_off, logits_off, total;
 };
 
 constexpr int kPrefixSimtRows = 32;
@@ -58,6 +58,9 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
   const int64_t G = H / KVH, TG = T * G, rows = B * T * H, all = B * TG;
   pl.prefix_kernel = P <= 0 ? kSpanNone : kSpanSimt;
   pl.own_kernel = max_length <= 0 ? kSpanNone : kSpanSimt;
+  // unit and segment counts are 32-bit in the tensor-core kernels
+  if (B * KVH * T * G * ((P + 63) / 64 + (max_length + 63) / 64 + 2) >= (int64_t(1) << 31))
+    tensor_cores = false;
   if (tensor_cores && impl != PDB_PREFIX_SIMT) {
     if (pl.own_kernel) pl.own_kernel = kSpanMma;
     if (pl.prefix_kernel) {
@@ -76,9 +79,7 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
     s.kind = pdb::kPartUnits;
     s.R = 8 * pl.prefix_nt;
     s.segments = (int)((all + s.R - 1) / s.R);
-    s.overhead = pdb::kSpanOverhead;
-    s.seg_units = (int)((P + 63) / 64) + s.overhead;
-    const int64_t units = KVH * s.segments * (int64_t)s.seg_units;
+    const int64_t units = KVH * s.segments * ((P + 63) / 64 + pdb::kSpanOverhead);
     s.grid = (int)std::min<int64_t>(kSpanCtasPerSm * (int64_t)sms, units);
     prefix_parts = (size_t)(KVH * s.segments + s.grid) * s.R;
   } else if (pl.prefix_kernel == kSpanTc) {
@@ -87,8 +88,7 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
     s.R = 256;
     s.half = (int)(128 / G);
     s.segments = (int)((B * T + 2 * s.half - 1) / (2 * s.half));
-    s.seg_units = (int)((P + 127) / 128);
-    const int64_t units = KVH * s.segments * (int64_t)s.seg_units;
+    const int64_t units = KVH * s.segments * ((P + 127) / 128);
     s.grid = (int)std::min<int64_t>(sms, units);
     prefix_parts = (size_t)(KVH * s.segments + s.grid) * s.R;
   }
@@ -102,8 +102,7 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
     s.kind = pdb::kPartUnits;
     s.R = 8 * pl.own_nt;
     s.segments = (int)((TG + s.R - 1) / s.R);
-    s.overhead = pdb::kSpanOverhead;
-    const int64_t units = B * KVH * s.segments * ((max_length + 63) / 64 + s.overhead);
+    const int64_t units = B * KVH * s.segments * ((max_length + 63) / 64 + pdb::kSpanOverhead);
     s.grid = (int)std::min<int64_t>(kSpanCtasPerSm * (int64_t)sms, units);
     own_parts = (size_t)(B * KVH * s.segments + s.grid) * s.R;
   }
@@ -117,7 +116,8 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
   pl.prefix_o = take(prefix_parts * D * sizeof(float));
   pl.own_ml = take(own_parts * sizeof(float2));
   pl.own_o = take(own_parts * D * sizeof(float));
-  pl.start_off = take(pl.own_kernel == kSpanMma ? (size_t)(B + 1) * sizeof(int64_t) : 0);
+  pl.prefix_dir = take((size_t)(KVH * pl.prefix.segments) * sizeof(int2));
+  pl.own_dir = take((size_t)(B * KVH * pl.own.segments) * sizeof(int2));
   pl.lse_off = take(scored ? (size_t)rows * sizeof(float) : 0);
   pl.logits_off = take(scored ? (size_t)rows * (size_t)max_length * sizeof(float) : 0);
   pl.total = at;
@@ -158,10 +158,11 @@ cudaError_t launch_spans_simt(int dev, int dtype, const pdb::PrefixParams& p, bo
   return launch_prefix_simt_rows<float, 256>(dev, p, prefix, st);
 }
 
-template <int D, int NT>
+// ROWS 8, 16, 32 (NT tiles of 8 per warp, RW row groups).
+template <int D, int NT, int RW>
 cudaError_t launch_span_mma(int dev, const pdb::PrefixParams& p, const pdb::SpanSet& ss, int grid,
                             cudaStream_t st, const CUtensorMap& kmap, const CUtensorMap& vmap) {
-  using C = pdb::SpanMma<D, NT, D == 64 ? 2 : 1, (D == 128 && NT == 4) ? 2 : 3, true>;
+  using C = pdb::SpanMma<D, NT, RW, (D == 128 && RW == 2) ? 2 : 3, NT == 1>;
   auto* fn = &pdb::prefix_span_kernel<C>;
   if (ctas_per_sm(dev, reinterpret_cast<const void*>(fn), C::SMEM, C::THREADS) <= 0)
     return cudaErrorInvalidConfiguration;
@@ -177,16 +178,31 @@ cudaError_t launch_spans_mma(int dev, const pdb::PrefixParams& p, const PrefixPl
   ss.nseq = prefix ? 1 : p.B;
   ss.tokens = prefix ? p.B * p.T : p.T;
   ss.rows = ss.tokens * p.G;
-  ss.start = p.own_start;
+  ss.beside = !prefix && pl.prefix_kernel == kSpanTc;
   const int nt = prefix ? pl.prefix_nt : pl.own_nt, grid = ss.part.grid;
   if (p.D == 64) {
-    if (nt == 1) return launch_span_mma<64, 1>(dev, p, ss, grid, st, kmap, vmap);
-    if (nt == 2) return launch_span_mma<64, 2>(dev, p, ss, grid, st, kmap, vmap);
-    return launch_span_mma<64, 4>(dev, p, ss, grid, st, kmap, vmap);
+    if (nt == 1) return launch_span_mma<64, 1, 1>(dev, p, ss, grid, st, kmap, vmap);
+    if (nt == 2) return launch_span_mma<64, 2, 1>(dev, p, ss, grid, st, kmap, vmap);
+    return launch_span_mma<64, 2, 2>(dev, p, ss, grid, st, kmap, vmap);
   }
-  if (nt == 1) return launch_span_mma<128, 1>(dev, p, ss, grid, st, kmap, vmap);
-  if (nt == 2) return launch_span_mma<128, 2>(dev, p, ss, grid, st, kmap, vmap);
-  return launch_span_mma<128, 4>(dev, p, ss, grid, st, kmap, vmap);
+  if (nt == 1) return launch_span_mma<128, 1, 1>(dev, p, ss, grid, st, kmap, vmap);
+  if (nt == 2) return launch_span_mma<128, 2, 1>(dev, p, ss, grid, st, kmap, vmap);
+  return launch_span_mma<128, 2, 2>(dev, p, ss, grid, st, kmap, vmap);
+}
+
+// Pool [N, bs, KVH, D] as [64 columns, N * bs rows, D / 64 halves, KVH]; box = one
+// 16-token unit of one kv head, all its columns, half by half; 128-byte swizzle.
+bool encode_unit_map(CUtensorMap* m, const void* pool, int64_t N, int64_t bs, int64_t KVH,
+                     int64_t D) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  const cuuint64_t dims[4] = {64, (cuuint64_t)(N * bs), (cuuint64_t)(D / 64), (cuuint64_t)KVH};
+  const cuuint64_t strides[3] = {(cuuint64_t)(KVH * D * 2), 128, (cuuint64_t)(D * 2)};
+  const cuuint32_t box[4] = {64, (cuuint32_t)pdb::kUnitTokens, (cuuint32_t)(D / 64), 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pool), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Query tiles of the tcgen05 kernel: box {64 columns, G heads, `tokens` tokens}.
@@ -218,7 +234,8 @@ cudaError_t launch_prefix_tc(int dev, const pdb::PrefixParams& p, cudaStream_t s
   t.H = p.H; t.KVH = p.KVH; t.G = p.G;
   t.per_tile = p.prefix.half;
   t.pairs = p.prefix.segments;
-  t.key_tiles = p.prefix.seg_units;
+  t.key_tiles = (p.prefix_length + C::BN - 1) / C::BN;
+  t.dir = p.prefix.dir;
   t.prefix_length = p.prefix_length;
   t.block_size = p.block_size; t.bs_shift = p.bs_shift;
   t.scale_log2 = p.scale_log2;
@@ -240,7 +257,7 @@ bool prefix_sizes_ok(int64_t B, int64_t T, int64_t H, int64_t D, int64_t KVH, in
                      int64_t max_length) {
   const int64_t lim = int64_t(1) << 30;
   return B <= 65535 && T <= 4096 && H <= 4096 && KVH <= 65535 && P <= lim && max_length <= lim &&
-         B * T * H * D < (int64_t(1) << 40) && B * T * H < (int64_t(1) << 31);
+         B * T * H * D < (int64_t(1) << 40) && B * T * H < (int64_t(1) << 30);
 }
 
 }  // namespace
@@ -334,7 +351,8 @@ int pdb_shared_prefix_attention_impl(
   p.own = pl.own;
   p.own.ml = reinterpret_cast<float2*>(wb + pl.own_ml);
   p.own.o = reinterpret_cast<float*>(wb + pl.own_o);
-  p.own_start = reinterpret_cast<int64_t*>(wb + pl.start_off);
+  p.prefix.dir = reinterpret_cast<int2*>(wb + pl.prefix_dir);
+  p.own.dir = reinterpret_cast<int2*>(wb + pl.own_dir);
   if (scores) {
     p.lse = reinterpret_cast<float*>(wb + pl.lse_off);
     p.logits = reinterpret_cast<float*>(wb + pl.logits_off);
@@ -348,20 +366,24 @@ int pdb_shared_prefix_attention_impl(
   p.table_width = (int)table_width;
   p.prefix_length = (int)prefix_length; p.max_length = (int)max_length;
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
-  CUtensorMap kmap, vmap;
-  if (tensor_cores && !(encode_pool_map(&kmap, k_pool, num_blocks, block_size, kv_heads, head_dim) &&
-                        encode_pool_map(&vmap, v_pool, num_blocks, block_size, kv_heads, head_dim)))
+  CUtensorMap kmap, vmap, kunits, vunits;  // boxes of the tcgen05 kernel, of the mma.sync kernel
+  const bool tc = pl.prefix_kernel == kSpanTc;
+  const bool mma = pl.prefix_kernel == kSpanMma || pl.own_kernel == kSpanMma;
+  if ((tc && !(encode_pool_map(&kmap, k_pool, num_blocks, block_size, kv_heads, head_dim) &&
+               encode_pool_map(&vmap, v_pool, num_blocks, block_size, kv_heads, head_dim))) ||
+      (mma && !(encode_unit_map(&kunits, k_pool, num_blocks, block_size, kv_heads, head_dim) &&
+                encode_unit_map(&vunits, v_pool, num_blocks, block_size, kv_heads, head_dim))))
     return fail(PDB_ERR_CUDA, "cuTensorMapEncodeTiled failed for the KV pools");
   cudaError_t e = cudaSuccess;
   if (pl.prefix_kernel == kSpanTc)
     e = head_dim == 64 ? launch_prefix_tc<64>(dev, p, st, kmap, vmap)
                        : launch_prefix_tc<128>(dev, p, st, kmap, vmap);
   else if (pl.prefix_kernel == kSpanMma)
-    e = launch_spans_mma(dev, p, pl, true, st, kmap, vmap);
+    e = launch_spans_mma(dev, p, pl, true, st, kunits, vunits);
   else if (pl.prefix_kernel == kSpanSimt)
     e = launch_spans_simt(dev, dtype, p, true, st);
   if (e == cudaSuccess && pl.own_kernel == kSpanMma)
-    e = launch_spans_mma(dev, p, pl, false, st, kmap, vmap);
+    e = launch_spans_mma(dev, p, pl, false, st, kunits, vunits);
   else if (e == cudaSuccess && pl.own_kernel == kSpanSimt)
     e = launch_spans_simt(dev, dtype, p, false, st);
   if (e == cudaSuccess) {

@@ -21,7 +21,8 @@
 //     of rows), cut into one contiguous range per CTA; CTA c's piece of segment
 //     s is stored as piece s + c (distinct for distinct pieces, as each step to
 //     the next piece raises s, c or both), part index = piece * R + row of the
-//     segment. The pieces of a segment are those of consecutive CTAs.
+//     segment. The pieces of a segment are those of consecutive CTAs; the first
+//     and the last of them are noted in `dir`.
 // Either way a row's partials are evenly spaced: prefix_join_kernel joins them.
 #pragma once
 
@@ -29,10 +30,16 @@
 
 namespace pdb {
 
-// CTAs that share `units`: each has at least one, so that the pieces of a
-// segment are those of consecutive CTAs.
-__host__ __device__ __forceinline__ int64_t unit_ctas(int64_t units, int64_t grid) {
+// `units` cut into one range per CTA, lengths equal up to one; CTAs that share
+// them each have at least one, so the pieces of a segment are those of
+// consecutive CTAs. First unit of CTA c (of `ctas`; c = ctas: the end).
+__host__ __device__ __forceinline__ int unit_ctas(int units, int grid) {
   return units < grid ? units : grid;
+}
+__device__ __forceinline__ int unit_begin(int c, int units, int ctas) {
+  if (c >= ctas) return units;
+  const unsigned per = (unsigned)units / (unsigned)ctas, more = (unsigned)units - per * ctas;
+  return c * (int)per + (c < (int)more ? c : (int)more);
 }
 
 enum : int { kPartNone = 0, kPartSlots = 1, kPartUnits = 2 };
@@ -40,15 +47,13 @@ enum : int { kPartNone = 0, kPartSlots = 1, kPartUnits = 2 };
 struct PartSet {
   float2* ml;
   float* o;
+  int2* dir;          // kPartUnits: [segments of all sequences and kv heads] first, last CTA
   int kind;
   int slots, chunk;   // kPartSlots: key ranges [i * chunk, (i + 1) * chunk)
   int R;              // kPartUnits: rows of a segment
-  int tokens;         //   tokens (all G heads of a kv head) that a segment's rows hold
   int half;           //   tokens of its first R / 2 rows (two query tiles), or 0: rows are dense
   int segments;       //   segments per (sequence,) kv head
   int grid;           //   CTAs that share the units
-  int seg_units;      //   units of a segment of the prefix
-  int overhead;       //   of them at its start that hold no keys
 };
 
 struct PrefixParams {
@@ -61,7 +66,6 @@ struct PrefixParams {
   const int32_t* counts;        // [B] or NULL (all T)
   void* out;                    // [B, T, H, D]
   PartSet prefix, own;          // partials
-  int64_t* own_start;           // [B + 1] first unit of each sequence (tensor-core kernel)
   float* lse;                   // [rows] base-2 log of the softmax's denominator (scores only)
   float* logits;                // [B, KVH, logits_width, T G] base-2 logits of own tokens, or NULL
   const float* scores;          // [B, KVH, scores_width]
@@ -257,25 +261,21 @@ struct PartRange {
   int64_t at, step;
   int count;
 };
-__device__ __forceinline__ PartRange prefix_parts(const PartSet& s, int64_t rows, int64_t row,
-                                                  int used_slots, int64_t seg, int64_t first_unit,
-                                                  int64_t last_unit, int64_t units, int lr) {
-  if (s.kind == kPartSlots) return PartRange{row, rows, used_slots};
-  const int64_t ctas = unit_ctas(units, s.grid);
-  const int64_t c0 = part_owner(first_unit, units, ctas), c1 = part_owner(last_unit, units, ctas);
-  return PartRange{(seg + c0) * s.R + lr, s.R, (int)(c1 - c0) + 1};
-}
-// Row of token `t` (of those that share segments) and head g of the group: its
-// segment among them and its row there.
-__device__ __forceinline__ int prefix_segment(const PartSet& s, int64_t t, int g, int G, int* lr) {
+// Token t (of those that share segments), head g of the group: the row of its
+// segment; `seg` becomes the segment's index (it comes in as that of the first).
+__device__ __forceinline__ PartRange prefix_parts(const PartSet& s, int seg, int t, int g, int G) {
+  int lr;
   if (s.half) {  // two query tiles of R / 2 rows, each with a remainder of unused rows
-    const int seg = (int)(t / (2 * s.half)), in = (int)(t - (int64_t)seg * 2 * s.half);
-    *lr = (in / s.half) * (s.R / 2) + (in % s.half) * G + g;
-    return seg;
+    const int x = t / s.half, in = t - x * s.half;
+    seg += x >> 1;
+    lr = (x & 1) * (s.R / 2) + in * G + g;
+  } else {
+    const int r = t * G + g, x = r / s.R;
+    seg += x;
+    lr = r - x * s.R;
   }
-  const int64_t r = t * G + g;
-  *lr = (int)(r % s.R);
-  return (int)(r / s.R);
+  const int2 c = s.dir[seg];
+  return PartRange{(int64_t)(seg + c.x) * s.R + lr, s.R, c.y - c.x + 1};
 }
 
 // VEC: D % 4 == 0 and D <= 128, four dims per lane, LPR lanes per row (D / 4
@@ -286,40 +286,27 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
   grid_dependency_wait();
   launch_dependents();
   constexpr int NV = VEC ? 4 : 8;
-  int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  int row = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR);
   const int lane = threadIdx.x % LPR, D = p.D;
   const bool real = row < p.rows;  // the others follow along for the shuffles
-  if (!real) row = p.rows - 1;
-  const int64_t bt = row / p.H;
-  const int b = (int)(bt / p.T), t = (int)(bt % p.T), hq = (int)(row % p.H), h = hq / p.G,
-            g = hq % p.G;
+  if (!real) row = (int)p.rows - 1;
+  const int bt = row / p.H, b = bt / p.T, t = bt - b * p.T, hq = row - bt * p.H, h = hq / p.G,
+            g = hq - h * p.G;
   int n, count;
   prefix_sequence(p, b, n, count);
   const int limit = prefix_limit(n, count, t);
-  PartRange part[2] = {{0, 0, 0}, {0, 0, 0}};
+  PartRange part[2] = {{row, p.rows, 0}, {row, p.rows, 0}};
   if (limit >= 0 && p.prefix.kind) {
-    int lr = 0;
-    const int64_t seg = p.prefix.kind == kPartUnits
-                            ? (int64_t)h * p.prefix.segments + prefix_segment(p.prefix, bt, g, p.G, &lr)
-                            : 0;
-    const int64_t u = seg * p.prefix.seg_units;
-    part[0] = prefix_parts(p.prefix, p.rows, row, p.prefix.slots, seg, u + p.prefix.overhead,
-                           u + p.prefix.seg_units - 1,
-                           (int64_t)p.KVH * p.prefix.segments * p.prefix.seg_units, lr);
+    if (p.prefix.kind == kPartSlots)
+      part[0].count = p.prefix.slots;
+    else
+      part[0] = prefix_parts(p.prefix, h * p.prefix.segments, bt, g, p.G);
   }
-  if (limit > 0 && p.own.kind) {
-    int lr = 0;
-    int64_t in = 0, first = 0, last = 0, total = 0;
-    if (p.own.kind == kPartUnits) {
-      in = (int64_t)h * p.own.segments + prefix_segment(p.own, t, g, p.G, &lr);
-      const int keys = (n + 63) / 64;
-      first = p.own_start[b] + in * (keys + p.own.overhead) + p.own.overhead;
-      last = first + keys - 1;
-      total = p.own_start[p.B];
-    }
-    part[1] = prefix_parts(p.own, p.rows, row, p.own.kind == kPartSlots
-                                                   ? (limit + p.own.chunk - 1) / p.own.chunk : 0,
-                           (int64_t)b * p.KVH * p.own.segments + in, first, last, total, lr);
+  if (limit > 0) {
+    if (p.own.kind == kPartSlots)
+      part[1].count = (limit + p.own.chunk - 1) / p.own.chunk;
+    else
+      part[1] = prefix_parts(p.own, (b * p.KVH + h) * p.own.segments, t, g, p.G);
   }
   const float2* ml[2] = {p.prefix.ml, p.own.ml};
   const float* o[2] = {p.prefix.o, p.own.o};
@@ -335,7 +322,7 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
   for (int i = 0; i < NV; ++i) acc[i] = 0.f;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-#pragma unroll 4
+#pragma unroll 2
     for (int s = 0; s < part[x].count; ++s) {
       const int64_t at = part[x].at + s * part[x].step;
       const float2 v = ml[x][at];
@@ -358,7 +345,7 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
   }
   if (!real) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
-  T* out = static_cast<T*>(p.out) + row * D;
+  T* out = static_cast<T*>(p.out) + (int64_t)row * D;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int d = VEC ? 4 * lane + i : lane + 32 * i;

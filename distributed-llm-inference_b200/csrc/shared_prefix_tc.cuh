@@ -8,14 +8,15 @@
 // CTA of equal length: a CTA works on the end of one item and the start of the
 // next. CTA c's piece of item i is piece i + c of the partials.
 //
-// One CTA per SM, ten warps:
+// One CTA per SM, eleven warps:
 //   * warps 0-3 and 4-7: softmax of query tile 0 and 1, one row per thread: read
 //     the S row from TMEM, base-2 softmax against a running maximum that is
 //     raised only when a logit passes it by 2^8 (O in TMEM is rescaled then;
-//     exact after the final division), write P as FP16 over S in TMEM.
-//   * warp 8: TMA. K and V tiles (128 keys) go through one ring of buffers in the
-//     order K0 V0 K1 V1 ..; a piece's query tiles ride on its first K.
-//   * warp 9: MMA issuer (warp-uniform, one elected lane). Per key tile j:
+//     exact after the final division), write P as FP16 over half of S in TMEM.
+//   * warps 9 and 10: TMA, for K and for V (one warp issues a 16-row box every
+//     ~100 cycles, the TMA unit takes one every 61). K and V tiles (128 keys) go
+//     through one ring of buffers in the order K0 V0 K1 V1 ..
+//   * warp 8: MMA issuer (warp-uniform, one elected lane). Per key tile j:
 //     O0 += P0 V_j, S0 = Q0 K_{j+1}, O1 += P1 V_j, S1 = Q1 K_{j+1}: while one
 //     tile's rows are exponentiated the tensor cores work for the other.
 //     The MMAs of a CTA run in issue order, so S_{j+1} may overwrite P_j
@@ -29,13 +30,13 @@
 // the exponentials (2 x 128 x 128 at 16 a cycle = 2048 cycles) alike.
 #pragma once
 
-#include "prefill_tc.cuh"
-#include "shared_prefix.cuh"
+#include "shared_prefix_mma.cuh"
 
 namespace pdb {
 
 struct PrefixTcParams {
   const int32_t* table;
+  int2* dir;                  // [items] first, last CTA
   float2* ml;                 // [pieces][256]
   float* o;                   // [pieces][256][D]
   int64_t num_blocks;
@@ -54,11 +55,50 @@ struct PrefixTc {
   static constexpr int HALVES = D / 64, UNITS = BN / 16;
   static constexpr int Q_BYTES = BM * D * 2, KV_BYTES = BN * D * 2;
   static constexpr int BUFS = D == 128 ? 5 : 8;  // ring of K and V tiles
-  static constexpr int THREADS = 320;
+  static constexpr int THREADS = 352;
   static constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;
   static constexpr int NBARS = 2 * BUFS + 1 + 2 + 2 + 2 + 1;
   static constexpr size_t SMEM = 1024 + 2 * (size_t)Q_BYTES + (size_t)BUFS * KV_BYTES + NBARS * 8 + 16;
 };
+
+// Logits of keys at or past `valid` (of 64): -inf.
+__device__ __forceinline__ void mask64(uint32_t* s, int valid) {
+  if (valid < 64) {
+#pragma unroll
+    for (int x = 0; x < 64; ++x)
+      if (x >= valid) s[x] = __float_as_uint(-INFINITY);
+  }
+}
+__device__ __forceinline__ float max64(const uint32_t* s) {
+  float mx[8];
+#pragma unroll
+  for (int y = 0; y < 8; ++y) mx[y] = __uint_as_float(s[y]);
+#pragma unroll
+  for (int x = 8; x < 56; x += 16)
+#pragma unroll
+    for (int y = 0; y < 8; ++y)
+      mx[y] = fmax3(mx[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + 8 + y]));
+#pragma unroll
+  for (int y = 0; y < 8; ++y) mx[y] = fmaxf(mx[y], __uint_as_float(s[56 + y]));
+  return fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+}
+// pk = 2^(c s - ref) as FP16 pairs; returns their FP32 sum (of the unrounded weights).
+__device__ __forceinline__ float weights64(const uint32_t* s, uint32_t* pk, float c, float ref) {
+  const uint64_t c2 = f2(c, c), nm2 = f2(-ref, -ref);
+  uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+  for (int x = 0; x < 32; ++x) {
+    float y0, y1;
+    f2_split(ffma2(f2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), c2, nm2), y0, y1);
+    const float a = ex2(y0), b = ex2(y1);
+    sum[x & 3] = fadd2(sum[x & 3], f2(a, b));
+    pk[x] = pack_half2(a, b);
+  }
+  float r[8];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) f2_split(sum[x], r[2 * x], r[2 * x + 1]);
+  return ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7]));
+}
 
 template <int D>
 __global__ void __launch_bounds__(PrefixTc<D>::THREADS, 1)
@@ -83,6 +123,9 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
+    prefetch_tensormap(&qmap);
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
     for (int i = 0; i < BUFS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -111,79 +154,93 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
     if (live) live = mbar_wait(bar, parity);
   };
 
-  // this CTA's units [u, u1) of (item, key tile)
-  const int64_t units = (int64_t)p.KVH * p.pairs * p.key_tiles;
-  const int64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+  // this CTA's units [u0, u1) of (item, key tile)
+  const int units = p.KVH * p.pairs * p.key_tiles;
+  const int ctas = unit_ctas(units, (int)gridDim.x), me = (int)blockIdx.x;
+  const int u0 = unit_begin(me, units, ctas), u1 = unit_begin(me + 1, units, ctas);
   // Piece that starts at unit u: item, first key tile, number of key tiles.
-  auto piece = [&](int64_t u, int& item, int& j0, int& nj) {
-    item = (int)(u / p.key_tiles);
-    j0 = (int)(u - (int64_t)item * p.key_tiles);
-    const int64_t end = (int64_t)(item + 1) * p.key_tiles;
-    nj = (int)((end < u1 ? end : u1) - u);
+  auto piece = [&](int u, int& item, int& j0, int& nj) {
+    item = u / p.key_tiles;
+    j0 = u - item * p.key_tiles;
+    const int end = (item + 1) * p.key_tiles;
+    nj = (end < u1 ? end : u1) - u;
   };
   // Tiles that hold rows: a kv head's last pair may lack its second.
   auto tiles_of = [&](int pair) { return (2 * pair + 1) * p.per_tile < p.tokens ? 2 : 1; };
 
-  if (warp == 8) {
-    // ---- TMA ------------------------------------------------------------------
-    int g = 0, n = 0;  // ring position, pieces so far
+  if (warp >= 9) {
+    // ---- TMA: warp 9 the queries and K tiles, warp 10 the V tiles -------------------
+    const int kv = warp - 9;
+    const CUtensorMap* map = kv ? &vmap : &kmap;
+    int g = kv, n = 0;  // ring position (K and V alternate), pieces so far
     int item, j0, nj;
-    for (int64_t u = u0; u < u1; u += nj, ++n) {
+    // Pool row of this lane's unit of key tile j: -1 past the end or without a page.
+    auto look_up = [&](int j) -> int {
+      const int t = j * BN + lane * 16;
+      if (lane >= UNITS || t >= p.prefix_length) return -1;
+      const int pi = p.bs_shift >= 0 ? t >> p.bs_shift : t / p.block_size;
+      const int page = __ldg(p.table + pi);
+      if (page < 0 || (int64_t)page >= p.num_blocks) {
+        raise_error(0x1u);
+        return -1;
+      }
+      return page * p.block_size + (t - pi * p.block_size);
+    };
+    for (int u = u0; u < u1; u += nj, ++n) {
       piece(u, item, j0, nj);
       const int h = item / p.pairs, pair = item % p.pairs, nt = tiles_of(pair);
-      // the query buffers double as the epilogue's staging: free once it is done
-      if (n > 0) wait(piece_done, (uint32_t)(n - 1) & 1u);
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, (uint32_t)(nt * HALVES * p.per_tile * p.G * 128));
-        for (int i = 0; i < nt; ++i)
+      int next = look_up(j0);
+      if (kv == 0) {
+        // the query buffers double as the epilogue's staging: free once it is done
+        if (n > 0) wait(piece_done, (uint32_t)(n - 1) & 1u);
+        if (lane == 0) {
+          if (j0 == 0) p.dir[item].x = me;
+          if (j0 + nj == p.key_tiles) p.dir[item].y = me;
+          mbar_arrive_expect_tx(q_full, (uint32_t)(nt * HALVES * p.per_tile * p.G * 128));
+          for (int i = 0; i < nt; ++i)
 #pragma unroll
-          for (int hf = 0; hf < HALVES; ++hf)
-            tma_load_3d(sq(i) + hf * (BM * 128), &qmap, hf * 64, h * p.G,
-                        (2 * pair + i) * p.per_tile, q_full);
-      }
-      __syncwarp();
-      for (int j = j0; j < j0 + nj; ++j) {
-        int64_t cell = -1;
-        if (lane < UNITS && j * BN + lane * 16 < p.prefix_length) {
-          const int t = j * BN + lane * 16;
-          const int pi = p.bs_shift >= 0 ? t >> p.bs_shift : t / p.block_size;
-          const int page = __ldg(p.table + pi);
-          if (page < 0 || (int64_t)page >= p.num_blocks)
-            raise_error(0x1u);
-          else
-            cell = (int64_t)page * p.block_size + (t - pi * p.block_size);
+            for (int hf = 0; hf < HALVES; ++hf)
+              tma_load_3d(sq(i) + hf * (BM * 128), &qmap, hf * 64, h * p.G,
+                          (2 * pair + i) * p.per_tile, q_full);
         }
+        __syncwarp();
+      }
+      for (int j = j0; j < j0 + nj; ++j, g += 2) {
+        const int cell = next;
+        if (j + 1 < j0 + nj) next = look_up(j + 1);  // in flight while this tile is issued
         const unsigned ok = __ballot_sync(0xffffffffu, cell >= 0);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++g) {
-          const int b = g % BUFS;
-          if (g >= BUFS) wait(&empty[b], (uint32_t)(g / BUFS - 1) & 1u);
-          // units without a page (past the end, or bad): zeros
+        const int b = g % BUFS;
+        if (g >= BUFS) wait(&empty[b], (uint32_t)(g / BUFS - 1) & 1u);
+        if (ok != (1u << UNITS) - 1) {  // units without a page (past the end, or bad): zeros
           for (int i = lane; i < UNITS * 16 * (D / 8); i += 32) {
             const int row = i / (D / 8), c = i % (D / 8);
             if (!(ok >> (row >> 4) & 1))
               *reinterpret_cast<uint4*>(buf(b) + (c >> 3) * (BN * 128) + row * 128 +
                                         ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-            else
-              i += 16 * (D / 8) - 32;
           }
-          if (ok != (1u << UNITS) - 1) fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(&full[b], (uint32_t)__popc(ok) * HALVES * 2048u);
-          __syncwarp();
-          if (cell >= 0) {
+          fence_proxy_async_smem();
+        }
+        int from[UNITS];
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) from[i] = __shfl_sync(0xffffffffu, cell, i);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full[b], (uint32_t)__popc(ok) * HALVES * 2048u);
+#pragma unroll
+          for (int i = 0; i < UNITS; ++i) {
+            if (from[i] < 0) continue;
 #pragma unroll
             for (int hf = 0; hf < HALVES; ++hf)
-              tma_load_3d(buf(b) + hf * (BN * 128) + lane * 2048, kv ? &vmap : &kmap, hf * 64, h,
-                          (int)cell, &full[b]);
+              tma_load_3d(buf(b) + hf * (BN * 128) + i * 2048, map, hf * 64, h, from[i], &full[b]);
           }
         }
+        __syncwarp();
       }
     }
     // every commit to an `empty` barrier has arrived before the CTA ends
-    for (int gg = g > BUFS ? g - BUFS : 0; gg < g; ++gg)
+    const int used = g - kv;  // tiles of both kinds
+    for (int gg = used > BUFS ? used - BUFS : 0; gg < used; ++gg)
       wait(&empty[gg % BUFS], (uint32_t)(gg / BUFS) & 1u);
-  } else if (warp == 9) {
+  } else if (warp == 8) {
     // ---- MMA issuer -------------------------------------------------------------
     constexpr uint32_t IDESC_S = f16_idesc(BM, BN, 0, 0);
     constexpr uint32_t IDESC_O = f16_idesc(BM, D, 0, 1);
@@ -203,7 +260,7 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
     };
     int g = 0, n = 0, tile[2] = {0, 0};  // ring position, pieces, P tiles so far
     int item, j0, nj;
-    for (int64_t u = u0; u < u1; u += nj, ++n) {
+    for (int u = u0; u < u1; u += nj, ++n) {
       piece(u, item, j0, nj);
       const int nt = tiles_of(item % p.pairs);
       wait(q_full, (uint32_t)n & 1u);
@@ -219,19 +276,25 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
         const int vb = g % BUFS, kb = (g + 1) % BUFS;
         wait(&full[vb], (uint32_t)(g / BUFS) & 1u);
         const bool more = j + 1 < nj;
-        if (more) wait(&full[kb], (uint32_t)((g + 1) / BUFS) & 1u);
         for (int i = 0; i < nt; ++i) {
           wait(&p_full[i], (uint32_t)tile[i]++ & 1u);
           __syncwarp();
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk)
-            tc_mma_ts_elect(tmem + C::O_COL + i * 128, tmem + C::S_COL + i * 128 + kk * 8,
+            tc_mma_ts_elect(tmem + C::O_COL + i * 128, tmem + C::S_COL + i * 128 + 64 + kk * 8,
                             v_desc + vb * STEP + kk * (16 * 128 >> 4), IDESC_O,
                             (j > 0 || kk > 0) ? 1u : 0u);
           if (!more) tc_commit_elect(&o_full[i]);
           if (i == nt - 1) tc_commit_elect(&empty[vb]);
-          if (more) qk(i, kb);
+          if (more) {
+            if (i == 0) {
+              wait(&full[kb], (uint32_t)((g + 1) / BUFS) & 1u);
+              __syncwarp();
+              tc_fence_after();
+            }
+            qk(i, kb);
+          }
         }
         if (more) tc_commit_elect(&empty[kb]);
         g += more ? 2 : 1;
@@ -247,7 +310,7 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
     const float c = p.scale_log2;
     int n = 0, tile = 0, done = 0;  // pieces; this tile's S phases; its pieces
     int item, j0, nj;
-    for (int64_t u = u0; u < u1; u += nj, ++n) {
+    for (int u = u0; u < u1; u += nj, ++n) {
       piece(u, item, j0, nj);
       const int pair = item % p.pairs;
       if (i < tiles_of(pair)) {
@@ -255,30 +318,22 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
         for (int j = 0; j < nj; ++j, ++tile) {
           wait(&s_full[i], (uint32_t)tile & 1u);
           tc_fence_after();
-          uint32_t s[BN];
-#pragma unroll
-          for (int q = 0; q < BN / 32; ++q) tc_ld32(s_col + q * 32, s + q * 32);
-          tc_wait_ld();
-#pragma unroll
-          for (int q = 0; q < BN / 32; ++q) tc_reg_fence32(s + q * 32);
+          // Pass 1: the row's maximum. The second half of the logits stays in
+          // registers, the first is read again: 128 at once would not fit.
           const int valid = p.prefix_length - (j0 + j) * BN;
-          if (valid < BN) {
+          uint32_t s[64];
+          float top = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < BN; ++x)
-              if (x >= valid) s[x] = __float_as_uint(-INFINITY);
+          for (int hf = 0; hf < 2; ++hf) {
+            tc_ld32(s_col + hf * 64, s);
+            tc_ld32(s_col + hf * 64 + 32, s + 32);
+            tc_wait_ld();
+            tc_reg_fence32(s);
+            tc_reg_fence32(s + 32);
+            mask64(s, valid - hf * 64);
+            top = fmaxf(top, max64(s));
           }
-          float mx[8];
-#pragma unroll
-          for (int x = 0; x < 8; ++x) mx[x] = __uint_as_float(s[x]);
-#pragma unroll
-          for (int x = 8; x < BN; x += 16)
-#pragma unroll
-            for (int y = 0; y < 8; ++y)
-              mx[y] = x + 8 < BN ? fmax3(mx[y], __uint_as_float(s[x + y]),
-                                         __uint_as_float(s[(x + 8 < BN ? x + 8 : x) + y]))
-                                 : fmaxf(mx[y], __uint_as_float(s[x + y]));
-          const float top = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]),
-                                  fmaxf(mx[6], mx[7])) * c;
+          top *= c;
           float alpha = 1.f;
           if (top > m_used + 8.f) {
             alpha = ex2(m_used - top);
@@ -286,22 +341,20 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
           }
           // all logits -inf so far: any finite reference gives weights 0
           const float ref = m_used == -INFINITY ? 0.f : m_used;
-          const uint64_t c2 = f2(c, c), nm2 = f2(-ref, -ref);
-          uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
-          uint32_t pk[BN / 2];
-#pragma unroll
-          for (int x = 0; x < BN / 2; ++x) {
-            float y0, y1;
-            f2_split(ffma2(f2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), c2, nm2),
-                     y0, y1);
-            const float a = ex2(y0), b = ex2(y1);
-            sum[x & 3] = fadd2(sum[x & 3], f2(a, b));
-            pk[x] = pack_half2(a, b);
-          }
-          float r[8];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) f2_split(sum[x], r[2 * x], r[2 * x + 1]);
-          l = l * alpha + (((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7])));
+          // Pass 2: weights, second half first; P goes to columns 64 .. 127, whose
+          // logits are in registers by then.
+          uint32_t pk[32];
+          float sum = weights64(s, pk, c, ref);
+          tc_st32(s_col + 96, pk);
+          tc_ld32(s_col, s);
+          tc_ld32(s_col + 32, s + 32);
+          tc_wait_ld();
+          tc_reg_fence32(s);
+          tc_reg_fence32(s + 32);
+          mask64(s, valid);
+          sum += weights64(s, pk, c, ref);
+          tc_st32(s_col + 64, pk);
+          l = l * alpha + sum;
           if (valid < BN && i == 0) {
             // V rows past the prefix (stale cells of its last unit): zeros. K and V
             // alternate in the ring: this tile's V is buffer 2 * tile + 1.
@@ -328,8 +381,6 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
               tc_st32(o_col + q * 32, ov);
             }
           }
-          tc_st32(s_col, pk);
-          tc_st32(s_col + 32, pk + 32);
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -340,7 +391,7 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
         wait(&o_full[i], (uint32_t)done & 1u);
         ++done;
         tc_fence_after();
-        const int64_t at0 = ((int64_t)item + blockIdx.x) * (2 * BM) + i * BM + wq * 32;
+        const int64_t at0 = (int64_t)(item + me) * (2 * BM) + i * BM + wq * 32;
         const int token0 = (2 * pair + i) * p.per_tile;
         const int used_rows =
             (p.tokens - token0 < p.per_tile ? p.tokens - token0 : p.per_tile) * p.G;
