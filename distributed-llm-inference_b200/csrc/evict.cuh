@@ -9,9 +9,13 @@
 // evict_select_kernel: one CTA per (sequence, kv head). Scores become 32-bit
 // keys in the order of the floats; the threshold (the largest key that at
 // least m - r candidates reach) is found bit by bit from the top, counting the
-// candidates at or above a trial key: 32 counts over keys that stay in
-// registers, instead of histograms whose few busy bins serialise. Two block
-// scans then number the ties and the kept tokens in index order.
+// candidates at or above a trial key, until a count is exact. The first
+// kEvictWideBits bits count keys in registers; the keys that share those bits
+// with the threshold are then gathered in shared memory and only they are counted
+// on (histograms instead serialise on the few bins that scores of like magnitude
+// share). Counts per stripe of 32 scores, scanned once, number the ties and the
+// kept tokens in index order. Bound by instruction issue: 48 x 8 heads of up to
+// 8192 scores took 53 us with every bit counted over every key at one CTA per SM.
 // evict_move_kernel: copies rows in 16-byte pieces; bound by HBM.
 #pragma once
 
@@ -67,35 +71,47 @@ __device__ __forceinline__ int evict_block_sum(int v, int* red, int& turn) {
   // 16 words, each held by two lanes of the warp
   return __reduce_add_sync(0xffffffffu, s) >> 1;
 }
-// Exclusive prefix of `v` over the CTA's threads, and the CTA's sum.
-__device__ __forceinline__ int evict_block_scan(int v, int* red, int& turn, int* sum) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int inc = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += y;
-  }
-  int* r = red + turn * kEvictWarps;
-  turn ^= 1;
-  if (lane == 31) r[warp] = inc;
+// Counts per (stripe, warp), stripe-major, to their exclusive prefix in place;
+// returns their sum to every thread. Two barriers.
+template <int E>
+__device__ __forceinline__ int evict_scan_counts(int* counts) {
+  static_assert(E * kEvictWarps <= 32 * E && kEvictWarps == 16, "16 E counts, one warp");
   __syncthreads();
-  int before = 0, all = 0;
+  if (threadIdx.x < 32) {
+    constexpr int PER = E / 2;  // 16 E counts over 32 lanes
+    int v[PER], mine = 0;
 #pragma unroll
-  for (int w = 0; w < kEvictWarps; ++w) {
-    if (w < warp) before += r[w];
-    all += r[w];
+    for (int i = 0; i < PER; ++i) {
+      v[i] = counts[threadIdx.x * PER + i];
+      mine += v[i];
+    }
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if ((int)threadIdx.x >= o) inc += y;
+    }
+    int run = inc - mine;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      counts[threadIdx.x * PER + i] = run;
+      run += v[i];
+    }
+    if (threadIdx.x == 31) counts[16 * E] = inc;
   }
-  *sum = all;
-  return before + inc - v;
+  __syncthreads();
+  return counts[16 * E];
 }
 
-// Candidates per round of the CTA: E consecutive ones per thread.
+// Candidates per round of the CTA: E stripes of one per thread.
+constexpr int kEvictWideBits = 12, kEvictList = 2048;
 template <int E>
-__global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const EvictParams p) {
   __shared__ int red[2 * kEvictWarps];
+  __shared__ int tie_counts[16 * E + 1], keep_counts[16 * E + 1], list_n;
+  __shared__ uint32_t list[kEvictList];
   int turn = 0;
-  const int bh = blockIdx.x, b = bh / p.KVH, tid = threadIdx.x;
+  const int bh = blockIdx.x, b = bh / p.KVH, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dependency_wait();
   launch_dependents();
   const int n = evict_length(p, b);
@@ -108,20 +124,31 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
   if (tid == 0 && bh % p.KVH == 0) p.new_lengths[b] = m;
 
   constexpr int ROUND = kEvictThreads * E;
-  const bool one = cand <= ROUND;  // every key stays in registers
-  uint32_t key[E];
+  const bool one = cand <= ROUND;  // every score stays in registers
+  uint32_t key[E];  // 0 (below every real key) past the candidates
   auto load = [&](int base) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int j = base + tid * E + e;
-      key[e] = j < cand ? evict_key(__ldg(sc + j)) : 0u;
+      const int j = base + e * kEvictThreads + tid;
+      key[e] = j < cand ? __float_as_uint(__ldg(sc + j)) : 0u;
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      key[e] = base + e * kEvictThreads + tid < cand ? evict_key(__uint_as_float(key[e])) : 0u;
   };
+  if (one) load(0);
+  // what needs no selection
+  for (int i = tid; i < r; i += kEvictThreads) {
+    kept[want + i] = cand + i;
+    nsc[want + i] = sc[cand + i];
+  }
+  for (int64_t i = m + tid; i < p.S; i += kEvictThreads) nsc[i] = 0.f;
+  for (int i = m + tid; i < p.budget; i += kEvictThreads) kept[i] = -1;
   uint32_t thr = 0u;  // the largest key that at least `want` candidates reach
   if (want < cand) {  // want == cand keeps all: threshold 0
-    if (one) load(0);
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t trial = thr | (1u << bit);
+    bool exact = false;
+    int bit = 31, over = cand;  // candidates at or above thr
+    auto count = [&](uint32_t trial) {
       int c = 0;
       if (one) {
 #pragma unroll
@@ -129,71 +156,112 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
       } else {
         for (int j = tid; j < cand; j += kEvictThreads) c += evict_key(__ldg(sc + j)) >= trial;
       }
-      if (evict_block_sum(c, red, turn) >= want) thr = trial;
+      return evict_block_sum(c, red, turn);
+    };
+    auto step = [&](int c, uint32_t trial) {  // exactly `want` reach trial: keep keys > trial - 1
+      if (c == want) {
+        thr = trial - 1;
+        exact = true;
+      } else if (c > want) {
+        thr = trial;
+        over = c;
+      }
+    };
+    for (; bit >= 32 - kEvictWideBits && !exact; --bit)
+      step(count(thr | (1u << bit)), thr | (1u << bit));
+    // keys that share the bits so far: those in [thr, thr + 2^(bit + 1))
+    const uint32_t span = 1u << (bit + 1);
+    if (!exact) {
+      if (tid == 0) list_n = 0;
+      __syncthreads();
+      auto put = [&](uint32_t k) {
+        const bool in = k - thr < span && k != 0u;
+        const unsigned mask = __ballot_sync(0xffffffffu, in);
+        int at = 0;
+        if (lane == 0 && mask) at = atomicAdd(&list_n, __popc(mask));  // order does not matter
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
+        if (in && at < kEvictList) list[at] = k;
+      };
+      if (one) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) put(key[e]);
+      } else {
+        for (int j = tid; j - tid < cand; j += kEvictThreads)
+          put(j < cand ? evict_key(__ldg(sc + j)) : 0u);
+      }
+      __syncthreads();
+      const int ln = list_n, higher = over - ln;  // candidates above the list's range
+      const bool listed = ln <= kEvictList;
+      for (; bit >= 0 && !exact; --bit) {
+        const uint32_t trial = thr | (1u << bit);
+        if (listed) {
+          int c = 0;
+          for (int j = tid; j < ln; j += kEvictThreads) c += list[j] >= trial;
+          step(evict_block_sum(c, red, turn) + higher, trial);
+        } else {
+          step(count(trial), trial);
+        }
+      }
     }
   }
   // ties at the threshold that stay: the first `ties` of them
   int above = 0;
-  for (int base = 0; base < cand; base += ROUND) {
-    load(base);
-    int c = 0;
+  if (one) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) c += key[e] > thr;
-    above += evict_block_sum(c, red, turn);
+    for (int e = 0; e < E; ++e) above += key[e] > thr;
+  } else {
+    for (int j = tid; j < cand; j += kEvictThreads) above += evict_key(__ldg(sc + j)) > thr;
   }
-  const int ties = want - above;
+  const int ties = want - evict_block_sum(above, red, turn);
   int tie_base = 0, out_base = 0;
+  const unsigned below = (1u << lane) - 1;
   for (int base = 0; base < cand; base += ROUND) {
-    load(base);
-    int eq = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) eq += base + tid * E + e < cand && key[e] == thr;
-    int sum;
-    int tie = tie_base + evict_block_scan(eq, red, turn, &sum);
-    tie_base += sum;
-    unsigned keep = 0;
-    int c = 0;
+    if (!one) load(base);
+    unsigned eq[E], keep[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const bool in = base + tid * E + e < cand;
-      bool k = in && key[e] > thr;
-      if (in && key[e] == thr) k = tie++ < ties;
-      keep |= (unsigned)k << e;
-      c += k;
+      eq[e] = __ballot_sync(0xffffffffu, key[e] == thr && key[e] != 0u);
+      if (lane == 0) tie_counts[e * kEvictWarps + warp] = __popc(eq[e]);
     }
-    int at = out_base + evict_block_scan(c, red, turn, &sum);
-    out_base += sum;
+    const int tie_sum = evict_scan_counts<E>(tie_counts);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (keep >> e & 1u) {
-        const int j = base + tid * E + e;
+      const int rank = tie_base + tie_counts[e * kEvictWarps + warp] + __popc(eq[e] & below);
+      keep[e] = __ballot_sync(0xffffffffu, key[e] > thr || ((eq[e] >> lane & 1u) && rank < ties));
+      if (lane == 0) keep_counts[e * kEvictWarps + warp] = __popc(keep[e]);
+    }
+    const int keep_sum = evict_scan_counts<E>(keep_counts);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (keep[e] >> lane & 1u) {
+        const int at = out_base + keep_counts[e * kEvictWarps + warp] + __popc(keep[e] & below);
+        const int j = base + e * kEvictThreads + tid;
         kept[at] = j;
-        nsc[at] = sc[j];
-        ++at;
+        nsc[at] = __ldg(sc + j);
       }
     }
+    tie_base += tie_sum;
+    out_base += keep_sum;
   }
-  for (int i = tid; i < r; i += kEvictThreads) {
-    kept[want + i] = cand + i;
-    nsc[want + i] = sc[cand + i];
-  }
-  for (int64_t i = m + tid; i < p.S; i += kEvictThreads) nsc[i] = 0.f;
-  for (int i = m + tid; i < p.budget; i += kEvictThreads) kept[i] = -1;
 }
 
-// One CTA moves 32 kept cells of one sequence, all kv heads, K and V.
+// One CTA moves 32 kept cells of up to 8 kv heads of one sequence, K and V: the
+// cells are looked up once into shared memory, then the pieces of their rows are
+// copied with eight loads in flight per thread.
 // P: the piece that rows are copied in (16 bytes where they allow it).
-constexpr int kEvictCells = 32;
+constexpr int kEvictCells = 32, kEvictHeads = 8;
 template <typename P>
 __global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
-  __shared__ int64_t s_new[kEvictCells];
-  const int b = blockIdx.y, i0 = blockIdx.x * kEvictCells, tid = threadIdx.x;
+  __shared__ int64_t s_from[kEvictCells * kEvictHeads], s_new[kEvictCells];
+  const int b = blockIdx.y, i0 = blockIdx.x * kEvictCells, h0 = blockIdx.z * kEvictHeads;
+  const int tid = threadIdx.x;
   grid_dependency_wait();
   launch_dependents();
   const int n = evict_length(p, b);
   const int m = n < p.budget ? n : p.budget;
   if (i0 >= m) return;
   const int cells = m - i0 < kEvictCells ? m - i0 : kEvictCells;
+  const int heads = p.KVH - h0 < kEvictHeads ? p.KVH - h0 : kEvictHeads;
   auto cell = [&](const int32_t* table, int width, int t) -> int64_t {
     const int pi = p.bs_shift >= 0 ? t >> p.bs_shift : t / p.block_size;
     const int page = pi < width ? __ldg(table + pi) : -1;
@@ -201,20 +269,45 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
       raise_error(0x1u);
       return -1;
     }
-    return (int64_t)page * p.block_size + (t - pi * p.block_size);
+    return ((int64_t)page * p.block_size + (t - pi * p.block_size)) * p.KVH;
   };
-  if (tid < cells) s_new[tid] = cell(p.new_tables + (int64_t)b * p.W2, p.W2, i0 + tid);
+  {  // 256 = 32 cells x 8 heads: neighbouring threads take neighbouring kept tokens
+    const int i = tid % kEvictCells, h = tid / kEvictCells;
+    if (i < cells && h < heads) {
+      const int j = __ldg(p.kept + ((int64_t)b * p.KVH + h0 + h) * p.budget + i0 + i);
+      s_from[tid] = cell(p.tables + (int64_t)b * p.W, p.W, j);
+    }
+    if (h == 0 && i < cells) s_new[i] = cell(p.new_tables + (int64_t)b * p.W2, p.W2, i0 + i);
+  }
   __syncthreads();
-  const int per_cell = p.KVH * p.row_pieces, total = cells * per_cell;
-  P* pools[2] = {static_cast<P*>(p.k_pool), static_cast<P*>(p.v_pool)};
-  for (int x = tid; x < total; x += 256) {
-    const int i = x / per_cell, y = x % per_cell, h = y / p.row_pieces;
-    const int64_t to = s_new[i];
-    const int j = __ldg(p.kept + ((int64_t)b * p.KVH + h) * p.budget + i0 + i);
-    const int64_t from = cell(p.tables + (int64_t)b * p.W, p.W, j);
-    if (to < 0 || from < 0) continue;
+  const int rp = p.row_pieces, per_cell = heads * rp, total = cells * per_cell;
+  P* kp = static_cast<P*>(p.k_pool);
+  P* vp = static_cast<P*>(p.v_pool);
+  constexpr int U = 4;
+  for (int x0 = tid; x0 < total; x0 += 256 * U) {
+    P kx[U], vx[U];
+    int64_t to[U];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) pools[kv][to * per_cell + y] = pools[kv][from * per_cell + y];
+    for (int u = 0; u < U; ++u) {
+      const int x = x0 + u * 256;
+      to[u] = -1;
+      if (x < total) {
+        const int i = x / per_cell, y = x - i * per_cell, h = y / rp, c = y - h * rp;
+        const int64_t from = s_from[h * kEvictCells + i], dst = s_new[i];
+        if (from >= 0 && dst >= 0) {
+          const int64_t at = (from + h0 + h) * rp + c;
+          to[u] = (dst + h0 + h) * rp + c;
+          kx[u] = kp[at];
+          vx[u] = vp[at];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (to[u] >= 0) {
+        kp[to[u]] = kx[u];
+        vp[to[u]] = vx[u];
+      }
   }
 }
 

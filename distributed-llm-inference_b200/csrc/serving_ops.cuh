@@ -23,7 +23,7 @@ enum SpanKernel { kSpanNone = 0, kSpanSimt, kSpanMma, kSpanTc };
 
 struct PrefixPlan {
   int prefix_kernel, own_kernel;
-  int prefix_nt, own_nt;  // kSpanMma: 8-row tiles per segment
+  int nt;  // kSpanMma: 8-row tiles per segment
   pdb::PartSet prefix, own;
   size_t prefix_ml, prefix_o, prefix_dir, own_ml, own_o, own_dir, lse_off, logits_off, total;
 };
@@ -49,8 +49,32 @@ void split_keys(int64_t keys, int64_t tiles, int64_t want, int64_t least, pdb::P
 int span_nt(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
 constexpr int kSpanCtasPerSm = 2;
-// From this many rows on, a prefix goes to the tcgen05 kernel (128-row tiles).
-constexpr int64_t kTcRows = 64;
+// From this many rows on, a prefix goes to the tcgen05 kernel (128-row tiles);
+// below, it is one more key set of the mma.sync kernel's launch.
+constexpr int64_t kTcRows = 33;
+
+// SMs of the tcgen05 kernel when the mma.sync kernel runs beside it on the others:
+// the split with the earlier end by the measured rates (a unit of 256 rows x 128
+// keys takes an SM 2.3 us; 64 keys of own context its share of HBM, 0.74 us per 32
+// KB, and not less than 0.5; about 10 and 8 us pass before and after), or all SMs
+// one after the other where that ends no later. Own lengths are on the device:
+// half the bound is taken. (B200, one token for 64 sequences, prefix 4096: 67 us on
+// all SMs in turn, 43.5 with 40 SMs for the prefix; 20 rows of four times the
+// lengths: no difference.)
+int tc_sms(int sms, double tc_units, double own_units, int64_t D) {
+  const double tc = 2.3 * tc_units, own = own_units * (D == 128 ? 0.74 : 0.5);
+  const double in_turn = 10 + tc / sms + 6 + own / sms;
+  double best = in_turn;
+  int n = 0;
+  for (int x = 1; x < sms; ++x) {
+    const double a = 10 + tc / x, b = 8 + own / (sms - x), t = a > b ? a : b;
+    if (t < 0.95 * in_turn && t < best) {
+      best = t;
+      n = x;
+    }
+  }
+  return n;  // 0: in turn
+}
 
 PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, int64_t D, int64_t P,
                        int64_t max_length, bool scored, bool tensor_cores, int impl) {
@@ -69,19 +93,11 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
       pl.prefix_kernel = tc ? kSpanTc : kSpanMma;
     }
   }
-  size_t prefix_parts = 0, own_parts = 0;
+  size_t prefix_parts = 0, own_parts = 0, span_segments = 0;  // own_parts: of the mma.sync launch
+  int beside_sms = 0;
   if (pl.prefix_kernel == kSpanSimt) {
     split_keys(P, (all + simt_rows(all) - 1) / simt_rows(all) * KVH, 4 * (int64_t)sms, 64, &pl.prefix);
     prefix_parts = (size_t)pl.prefix.slots * rows;
-  } else if (pl.prefix_kernel == kSpanMma) {
-    pl.prefix_nt = span_nt(all);
-    pdb::PartSet& s = pl.prefix;
-    s.kind = pdb::kPartUnits;
-    s.R = 8 * pl.prefix_nt;
-    s.segments = (int)((all + s.R - 1) / s.R);
-    const int64_t units = KVH * s.segments * ((P + 63) / 64 + pdb::kSpanOverhead);
-    s.grid = (int)std::min<int64_t>(kSpanCtasPerSm * (int64_t)sms, units);
-    prefix_parts = (size_t)(KVH * s.segments + s.grid) * s.R;
   } else if (pl.prefix_kernel == kSpanTc) {
     pdb::PartSet& s = pl.prefix;
     s.kind = pdb::kPartUnits;
@@ -89,22 +105,47 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
     s.half = (int)(128 / G);
     s.segments = (int)((B * T + 2 * s.half - 1) / (2 * s.half));
     const int64_t units = KVH * s.segments * ((P + 127) / 128);
-    s.grid = (int)std::min<int64_t>(sms, units);
+    int n = 0;
+    if (pl.own_kernel == kSpanMma) {
+      const int64_t r = 8 * span_nt(TG);
+      n = tc_sms(sms, (double)units,
+                 (double)(B * KVH * ((TG + r - 1) / r)) * (max_length / 128.0 + 1), D);
+    }
+    beside_sms = n;
+    s.grid = (int)std::min<int64_t>(n ? n : sms, units);
     prefix_parts = (size_t)(KVH * s.segments + s.grid) * s.R;
   }
   if (pl.own_kernel == kSpanSimt) {
     split_keys(max_length, (TG + simt_rows(TG) - 1) / simt_rows(TG) * B * KVH, 8 * (int64_t)sms, 128,
                &pl.own);
     own_parts = (size_t)pl.own.slots * rows;
-  } else if (pl.own_kernel == kSpanMma) {
-    pl.own_nt = span_nt(TG);
-    pdb::PartSet& s = pl.own;
+  }
+  const bool prefix_mma = pl.prefix_kernel == kSpanMma, own_mma = pl.own_kernel == kSpanMma;
+  if (prefix_mma || own_mma) {  // one launch: the prefix's segments, then those of own contexts
+    pl.nt = span_nt(prefix_mma ? all : TG);
+    const int R = 8 * pl.nt;
+    pdb::PartSet s{};
     s.kind = pdb::kPartUnits;
-    s.R = 8 * pl.own_nt;
-    s.segments = (int)((TG + s.R - 1) / s.R);
-    const int64_t units = B * KVH * s.segments * ((max_length + 63) / 64 + pdb::kSpanOverhead);
-    s.grid = (int)std::min<int64_t>(kSpanCtasPerSm * (int64_t)sms, units);
-    own_parts = (size_t)(B * KVH * s.segments + s.grid) * s.R;
+    s.R = R;
+    int64_t units = 0, segments = 0;
+    if (prefix_mma) {
+      pl.prefix = s;
+      pl.prefix.segments = (int)((all + R - 1) / R);
+      segments = KVH * pl.prefix.segments;
+      units = segments * ((P + 63) / 64 + pdb::kSpanOverhead);
+    }
+    if (own_mma) {
+      pl.own = s;
+      pl.own.segments = (int)((TG + R - 1) / R);
+      pl.own.first = (int)segments;
+      segments += B * KVH * pl.own.segments;
+      units += B * KVH * pl.own.segments * ((max_length + 63) / 64 + pdb::kSpanOverhead);
+    }
+    const int grid = (int)std::min<int64_t>(kSpanCtasPerSm * (int64_t)(sms - beside_sms), units);
+    pl.prefix.grid = prefix_mma ? grid : pl.prefix.grid;
+    pl.own.grid = own_mma ? grid : pl.own.grid;
+    own_parts = (size_t)(segments + grid) * R;
+    span_segments = (size_t)segments;
   }
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -117,7 +158,12 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
   pl.own_ml = take(own_parts * sizeof(float2));
   pl.own_o = take(own_parts * D * sizeof(float));
   pl.prefix_dir = take((size_t)(KVH * pl.prefix.segments) * sizeof(int2));
-  pl.own_dir = take((size_t)(B * KVH * pl.own.segments) * sizeof(int2));
+  pl.own_dir = take(span_segments * sizeof(int2));
+  if (prefix_mma) {
+    pl.prefix_ml = pl.own_ml;
+    pl.prefix_o = pl.own_o;
+    pl.prefix_dir = pl.own_dir;
+  }
   pl.lse_off = take(scored ? (size_t)rows * sizeof(float) : 0);
   pl.logits_off = take(scored ? (size_t)rows * (size_t)max_length * sizeof(float) : 0);
   pl.total = at;
@@ -168,18 +214,15 @@ cudaError_t launch_span_mma(int dev, const pdb::PrefixParams& p, const pdb::Span
     return cudaErrorInvalidConfiguration;
   return launch_pdl(fn, dim3((unsigned)grid), dim3(C::THREADS), C::SMEM, st, p, ss, kmap, vmap);
 }
-cudaError_t launch_spans_mma(int dev, const pdb::PrefixParams& p, const PrefixPlan& pl, bool prefix,
+cudaError_t launch_spans_mma(int dev, const pdb::PrefixParams& p, const PrefixPlan& pl,
                              cudaStream_t st, const CUtensorMap& kmap, const CUtensorMap& vmap) {
   pdb::SpanSet ss{};
-  ss.part = prefix ? p.prefix : p.own;
-  ss.own = prefix ? 0 : 1;
-  ss.tables = prefix ? p.prefix_table : p.tables;
-  ss.width = prefix ? (p.prefix_length + p.block_size - 1) / p.block_size : p.table_width;
-  ss.nseq = prefix ? 1 : p.B;
-  ss.tokens = prefix ? p.B * p.T : p.T;
-  ss.rows = ss.tokens * p.G;
-  ss.beside = !prefix && pl.prefix_kernel == kSpanTc;
-  const int nt = prefix ? pl.prefix_nt : pl.own_nt, grid = ss.part.grid;
+  ss.has_prefix = pl.prefix_kernel == kSpanMma ? 1 : 0;
+  ss.nseq = pl.own_kernel == kSpanMma ? p.B : 0;
+  ss.part = ss.nseq ? p.own : p.prefix;
+  ss.prefix_segments = ss.has_prefix ? p.prefix.segments : 0;
+  ss.beside = pl.prefix_kernel == kSpanTc;
+  const int nt = pl.nt, grid = ss.part.grid;
   if (p.D == 64) {
     if (nt == 1) return launch_span_mma<64, 1, 1>(dev, p, ss, grid, st, kmap, vmap);
     if (nt == 2) return launch_span_mma<64, 2, 1>(dev, p, ss, grid, st, kmap, vmap);
@@ -378,12 +421,10 @@ int pdb_shared_prefix_attention_impl(
   if (pl.prefix_kernel == kSpanTc)
     e = head_dim == 64 ? launch_prefix_tc<64>(dev, p, st, kmap, vmap)
                        : launch_prefix_tc<128>(dev, p, st, kmap, vmap);
-  else if (pl.prefix_kernel == kSpanMma)
-    e = launch_spans_mma(dev, p, pl, true, st, kunits, vunits);
   else if (pl.prefix_kernel == kSpanSimt)
     e = launch_spans_simt(dev, dtype, p, true, st);
-  if (e == cudaSuccess && pl.own_kernel == kSpanMma)
-    e = launch_spans_mma(dev, p, pl, false, st, kunits, vunits);
+  if (e == cudaSuccess && mma)
+    e = launch_spans_mma(dev, p, pl, st, kunits, vunits);
   else if (e == cudaSuccess && pl.own_kernel == kSpanSimt)
     e = launch_spans_simt(dev, dtype, p, false, st);
   if (e == cudaSuccess) {
@@ -445,9 +486,11 @@ int pdb_verify_drafts(const int64_t* draft_tokens, const void* target_probs,
   int dev = 0;
   const int rc = current_device(&dev);
   if (rc) return rc;
-  // CTAs per sequence: enough for two per SM, but at least 2048 entries each
+  // CTAs per sequence: up to four per SM in all, each with 2048 entries at least (256
+  // rows of 100003: 41 us with 2 CTAs, 58 with 1, 45 with 4; one row of 49152: 7.0 us
+  // with 8, 15.8 with 1)
   int C = 1;
-  while (C < pdb::kVerifyMaxCluster && batch * C < 2 * (int64_t)sm_count(dev) &&
+  while (C < pdb::kVerifyMaxCluster && batch * C * 2 <= 4 * (int64_t)sm_count(dev) &&
          vocab / (2 * C) >= 2048)
     C *= 2;
   cudaLaunchConfig_t cfg = {};
@@ -519,7 +562,8 @@ int pdb_evict_tokens(void* k_pool, void* v_pool, const float* scores, int64_t sc
                       ? launch_pdl(pdb::evict_select_kernel<4>, sel, dim3(pdb::kEvictThreads), 0, st, p)
                       : launch_pdl(pdb::evict_select_kernel<16>, sel, dim3(pdb::kEvictThreads), 0, st, p);
   if (e == cudaSuccess) {
-    const dim3 grid((unsigned)((most + pdb::kEvictCells - 1) / pdb::kEvictCells), (unsigned)batch);
+    const dim3 grid((unsigned)((most + pdb::kEvictCells - 1) / pdb::kEvictCells), (unsigned)batch,
+                    (unsigned)((kv_heads + pdb::kEvictHeads - 1) / pdb::kEvictHeads));
     if (wide)
       e = launch_pdl(pdb::evict_move_kernel<uint4>, grid, dim3(256), 0, st, p);
     else if (esize == 2)

@@ -53,6 +53,7 @@ struct PartSet {
   int R;              // kPartUnits: rows of a segment
   int half;           //   tokens of its first R / 2 rows (two query tiles), or 0: rows are dense
   int segments;       //   segments per (sequence,) kv head
+  int first;          //   index of the first segment
   int grid;           //   CTAs that share the units
 };
 
@@ -300,13 +301,13 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
     if (p.prefix.kind == kPartSlots)
       part[0].count = p.prefix.slots;
     else
-      part[0] = prefix_parts(p.prefix, h * p.prefix.segments, bt, g, p.G);
+      part[0] = prefix_parts(p.prefix, p.prefix.first + h * p.prefix.segments, bt, g, p.G);
   }
   if (limit > 0) {
     if (p.own.kind == kPartSlots)
       part[1].count = (limit + p.own.chunk - 1) / p.own.chunk;
     else
-      part[1] = prefix_parts(p.own, (b * p.KVH + h) * p.own.segments, t, g, p.G);
+      part[1] = prefix_parts(p.own, p.own.first + (b * p.KVH + h) * p.own.segments, t, g, p.G);
   }
   const float2* ml[2] = {p.prefix.ml, p.own.ml};
   const float* o[2] = {p.prefix.o, p.own.o};

@@ -38,20 +38,21 @@
 
 namespace pdb {
 
-// What one launch covers: `nseq` key sets of `rows` rows each; set s belongs to
-// tokens s * tokens .. of the batch.
+// What one launch covers: key sets of B own contexts (rows T G each) and, before
+// them, the prefix (rows B T G) when it has few rows. Segments are numbered through
+// both: the prefix's first, then those of sequence 0, 1, ..
 struct SpanSet {
-  const int32_t* tables;  // [nseq, width]
-  PartSet part;
-  int nseq, width, tokens, rows;
-  int own;                // own tokens (lengths, counts, causal) or the prefix
-  int beside;             // the previous kernel in the stream is this call's prefix kernel, whose
-                          // CTAs let this one start only once all work before it was complete:
-                          // nothing here waits for it but the end
+  PartSet part;               // segments: per own context and kv head
+  int has_prefix, nseq;       // key sets: has_prefix + nseq
+  int prefix_segments;        // per kv head
+  int beside;                 // the previous kernel in the stream is this call's prefix kernel, whose
+                              // CTAs let this one start only once all work before it was complete:
+                              // nothing here waits for it but the end
 };
 
 struct SpanRec {  // one staged tile, producer -> math warps
-  int seq, h, row0, k0, kend, n, count, piece, qbuf, flags, okmask, pad_;
+  int seq;  // sequence, or -1: the prefix
+  int h, row0, rows, k0, kend, n, count, piece, qbuf, flags, okmask;
 };
 constexpr int kSpanFirst = 1, kSpanLast = 2, kSpanEnd = 4;
 
@@ -129,12 +130,13 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
   }
   if (!ss.beside) grid_dependency_wait();
   launch_dependents();
-  auto length_of = [&](int s) -> int2 {
-    int n = p.prefix_length, count = ss.tokens;
-    if (ss.own) prefix_sequence(p, s, n, count);
+  const int sets = ss.has_prefix + ss.nseq;
+  auto length_of = [&](int s) -> int2 {  // keys and tokens of key set s
+    int n = p.prefix_length, count = p.B * p.T;
+    if (s >= ss.has_prefix) prefix_sequence(p, s - ss.has_prefix, n, count);
     return make_int2(n, count);
   };
-  for (int i = tid; i < ss.nseq && i < C::LCAP; i += C::THREADS) lens[i] = length_of(i);
+  for (int i = tid; i < sets && i < C::LCAP; i += C::THREADS) lens[i] = length_of(i);
   __syncthreads();
   bool live = true;  // after one expired wait a thread stops waiting
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -144,22 +146,24 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
   if (warp == 4) {
     // ---- producer ------------------------------------------------------------
     auto set_length = [&](int s) -> int2 { return s < C::LCAP ? lens[s] : length_of(s); };
-    const int per = p.KVH * ss.part.segments;  // segments of a key set
+    // segments of a key set, and of those before it
+    const int own_per = p.KVH * ss.part.segments, prefix_per = p.KVH * ss.prefix_segments;
+    auto per = [&](int s) { return s < ss.has_prefix ? prefix_per : own_per; };
     auto set_units = [&](int s) -> int {
-      if (s >= ss.nseq) return 0;
+      if (s >= sets) return 0;
       const int n = set_length(s).x;
-      return n > 0 ? per * ((n + 63) / 64 + kSpanOverhead) : 0;
+      return n > 0 ? per(s) * ((n + 63) / 64 + kSpanOverhead) : 0;
     };
     int total = 0;
-    for (int s0 = 0; s0 < ss.nseq; s0 += 32)
+    for (int s0 = 0; s0 < sets; s0 += 32)
       total += (int)__reduce_add_sync(0xffffffffu, (unsigned)set_units(s0 + lane));
     const int ctas = unit_ctas(total, (int)gridDim.x), me = (int)blockIdx.x;
     const int u0 = unit_begin(me, total, ctas), u1 = unit_begin(me + 1, total, ctas);
-    int s = ss.nseq, n = 0, count = 0;
+    int s = sets, n = 0, count = 0;
     int u = total, in = 0;  // start of the current segment; its index in the key set
     if (u0 < u1) {
       int run = 0;
-      for (int s0 = 0; s0 < ss.nseq; s0 += 32) {
+      for (int s0 = 0; s0 < sets; s0 += 32) {
         const int w = set_units(s0 + lane);
         int inc = w;
 #pragma unroll
@@ -191,29 +195,33 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
       const int lo = u0 - u - kSpanOverhead, hi = u1 - u - kSpanOverhead;
       const int j0 = lo > 0 ? lo : 0, j1 = hi < keys ? hi : keys;
       if (j0 < j1) {
-        const int seg = s * per + in;
+        const bool own = s >= ss.has_prefix;
+        const int seq = own ? s - ss.has_prefix : -1;
+        const int seg = (own ? ss.has_prefix * prefix_per + seq * own_per : 0) + in;
+        const int segments = own ? ss.part.segments : ss.prefix_segments;
+        const int token0 = own ? seq * p.T : 0, rows = (own ? p.T : p.B * p.T) * p.G;
+        const int32_t* table = own ? p.tables + (int64_t)seq * p.table_width : p.prefix_table;
+        const int width = own ? p.table_width : (p.prefix_length + p.block_size - 1) / p.block_size;
         if (lane == 0 && j0 == 0) ss.part.dir[seg].x = me;
         if (lane == 0 && j1 == keys) ss.part.dir[seg].y = me;
-        const int h = in / ss.part.segments, row0 = (in - h * ss.part.segments) * ROWS;
-        const int nrows = ss.rows - row0 < ROWS ? ss.rows - row0 : ROWS;
+        const int h = in / segments, row0 = (in - h * segments) * ROWS;
+        const int nrows = rows - row0 < ROWS ? rows - row0 : ROWS;
         const int k0 = j0 * 64, kend = j1 * 64 < n ? j1 * 64 : n;
         const int qb = item & 1;
         if (item >= 2) wait(&q_empty[qb], (uint32_t)((item >> 1) - 1) & 1u);
-        const int32_t* table = ss.tables + (int64_t)s * ss.width;
         for (int t0 = k0; t0 < kend; t0 += TILE, ++g) {
           const int st = (int)(g % STAGES);
           int64_t cell = -1;  // looked up before the wait: the page read hides behind it
           if (lane < UNITS && t0 + lane * 16 < kend)
-            cell = prefix_cell(p, table, ss.width, t0 + lane * 16);
+            cell = prefix_cell(p, table, width, t0 + lane * 16);
           if (g >= STAGES) wait(&empty[st], (uint32_t)(g / STAGES - 1) & 1u);
           const unsigned ok = __ballot_sync(0xffffffffu, cell >= 0);
           const bool first = t0 == k0;
           if (lane == 0) {
             SpanRec r;
-            r.seq = s; r.h = h; r.row0 = row0; r.k0 = t0; r.kend = kend; r.n = n; r.count = count;
+            r.seq = seq; r.h = h; r.row0 = row0; r.rows = rows; r.k0 = t0; r.kend = kend; r.n = n; r.count = count;
             r.piece = seg + me; r.qbuf = qb; r.okmask = (int)ok;
             r.flags = (first ? kSpanFirst : 0) | (t0 + TILE >= kend ? kSpanLast : 0);
-            r.pad_ = 0;
             recs[st] = r;
             mbar_arrive_expect_tx(&full[st], (uint32_t)__popc(ok) * 2u * C::UNIT_BYTES +
                                                  (first ? (uint32_t)nrows * D * 2u : 0u));
@@ -223,7 +231,7 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
             for (int r = lane; r < nrows; r += 32) {
               const int row = row0 + r;
               const __half* src = static_cast<const __half*>(p.q) +
-                                  (((int64_t)s * ss.tokens + row / p.G) * p.H + (int64_t)h * p.G +
+                                  ((int64_t)(token0 + row / p.G) * p.H + (int64_t)h * p.G +
                                    row % p.G) * D;
               bulk_load(sq + qb * C::Q_BYTES + r * C::QP, src, D * 2, &full[st]);
             }
@@ -244,10 +252,10 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
         ++item;
       }
       u += keys + kSpanOverhead;
-      if (++in == per) {  // next key set that holds keys
+      if (++in == per(s)) {  // next key set that holds keys
         in = 0;
         n = 0;
-        while (n <= 0 && ++s < ss.nseq) {
+        while (n <= 0 && ++s < sets) {
           const int2 nc = set_length(s);
           n = nc.x;
           count = nc.y;
@@ -288,7 +296,7 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
       r = recs[st];
       if (r.flags & kSpanEnd || !live) break;
     } else {
-      r.seq = r.h = r.row0 = r.k0 = r.piece = r.qbuf = r.count = 0;
+      r.seq = r.h = r.row0 = r.rows = r.k0 = r.piece = r.qbuf = r.count = 0;
       r.kend = r.n = TILE;
       r.flags = kSpanFirst;
       r.okmask = -1;
@@ -341,7 +349,7 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
       }
       // scale, mask
       const int key0 = r.k0 + w0 + gq;
-      const bool causal = ss.own && r.count > 1 && r.k0 + w0 + 16 * KB > r.n - r.count + 1;
+      const bool causal = r.seq >= 0 && r.count > 1 && r.k0 + w0 + 16 * KB > r.n - r.count + 1;
       const unsigned units = (unsigned)r.okmask >> (kw * KB);
       const bool edge = left < 16 * KB || causal || (units & ((1u << KB) - 1)) != (1u << KB) - 1;
       // V fragments: keys 2 tg, 2 tg + 1 (low, high half) and those 8 on
@@ -384,8 +392,8 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
           }
         }
       }
-      if (p.logits && ss.own && g >= 0) {
-        float* lg = p.logits + ((int64_t)r.seq * p.KVH + r.h) * p.logits_width * ss.rows;
+      if (p.logits && r.seq >= 0 && g >= 0) {
+        float* lg = p.logits + ((int64_t)r.seq * p.KVH + r.h) * p.logits_width * r.rows;
 #pragma unroll
         for (int sb = 0; sb < KB; ++sb)
 #pragma unroll
@@ -395,14 +403,14 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
 #pragma unroll
               for (int i = 0; i < NT; ++i) {
                 const int row = r.row0 + rows0 + 8 * i + 2 * tg;
-                float* at = lg + (int64_t)key * ss.rows + row;
-                if (ss.rows % 2 == 0) {
-                  if (row < ss.rows)
+                float* at = lg + (int64_t)key * r.rows + row;
+                if (r.rows % 2 == 0) {
+                  if (row < r.rows)
                     *reinterpret_cast<float2*>(at) =
                         make_float2(sc[sb][i][2 * e2], sc[sb][i][2 * e2 + 1]);
                 } else {
-                  if (row < ss.rows) at[0] = sc[sb][i][2 * e2];
-                  if (row + 1 < ss.rows) at[1] = sc[sb][i][2 * e2 + 1];
+                  if (row < r.rows) at[0] = sc[sb][i][2 * e2];
+                  if (row + 1 < r.rows) at[1] = sc[sb][i][2 * e2 + 1];
                 }
               }
             }
@@ -558,7 +566,7 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
       const int jr = tid / TPR, part = tid % TPR;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        if (r.row0 + 8 * i >= ss.rows) break;  // CTA-uniform
+        if (r.row0 + 8 * i >= r.rows) break;  // CTA-uniform
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int row = rows0 + 8 * i + 2 * tg + e;
@@ -576,7 +584,7 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
         }
         named_bar_sync(1, 128);
         const int lrow = (jr >> 3) * 8 * NT + 8 * i + (jr & 7);  // row of the segment
-        if (r.row0 + lrow < ss.rows) {
+        if (r.row0 + lrow < r.rows) {
           const int64_t at = (int64_t)r.piece * ROWS + lrow;
           float* og = ss.part.o + at * D;
 #pragma unroll

@@ -13,14 +13,15 @@
 // as none). A row whose w are all zero (p_a = q_a up to rounding) falls back
 // to p_a; a row without any weight gives token -1.
 //
-// One cluster of C CTAs per sequence, no workspace and no atomics. Every warp
-// of the cluster owns a contiguous segment of the vocabulary: (1) each warp
-// sums its segment, (2) the cluster reads all segment sums through distributed
-// shared memory and finds the segment that holds the level, (3) its CTA splits
-// that segment over its warps the same way and the warp that holds the level
-// scans 32 entries at a time. The row is read once from HBM (twice the chosen
-// segment, from L2). Bound by HBM at large batches, by the chain of three
-// dependent reads at small ones.
+// One cluster of C CTAs per sequence, no workspace and no atomics. Each CTA owns
+// a contiguous range of the vocabulary, cut into blocks of 256 K entries that its
+// warps take in turn, so that a CTA reads adjacent memory at any time: (1) every
+// block's sum goes to shared memory, the CTA's total to every CTA of the cluster
+// through distributed shared memory, (2) the totals give the CTA that holds the
+// level, its block sums the block, and one warp scans that block. The row is read
+// once from HBM (one block twice, from L2). Bound by HBM at large batches, by the
+// chain of dependent reads (draft, its probabilities, the row, the block) at small
+// ones.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -42,103 +43,174 @@ struct VerifyParams {
   int B, T;
 };
 
-constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyMaxCluster = 8;
+constexpr int kVerifyThreads = 256, kVerifyMaxCluster = 8;
+constexpr int kVerifyBlocks = 512;  // block sums that a CTA keeps
 
 // One row's weights: w_j = p_j - q_j, or p_j with entry `hit` taken out.
 template <typename T>
 struct VerifyRow {
   const T* p;
   const T* q;
-  int64_t hit;
-  __device__ __forceinline__ long long weight(float pj, float qj, int64_t j) const {
-    float w = __fsub_rn(pj, qj);  // NaN and negative differences count as none
-    if (j == hit) w = 0.f;
-    return w > 0.f ? __float2ll_rz(fminf(w, 1.f) * 1099511627776.f) : 0ll;
+  int hit;
+  bool wide;  // both rows 16-byte aligned
+  // The weight in units of 2^-40, in two parts of 20 bits: w = saturate(p - q) (NaN
+  // to 0), h = floor(w 2^20), l = floor((w 2^20 - h) 2^20), each read from the
+  // mantissa of a sum with 2^23 that is rounded down. Seven instructions; a conversion
+  // to a 64-bit integer with its clamps and sums takes more than twice that and
+  // bounds the kernel by issue (256 rows of 100003: 43 us).
+  static constexpr uint32_t kBias = 0x4B000000u;  // bits of 2^23
+  static __device__ __forceinline__ void add(float w, uint32_t& h, uint32_t& l) {
+    const float t = __fmaf_rd(w, 1048576.f, 8388608.f);
+    const float r = __fmaf_rn(w, 1048576.f, -__fsub_rn(t, 8388608.f));  // exact
+    h += __float_as_uint(t);
+    l += __float_as_uint(__fmaf_rd(r, 1048576.f, 8388608.f));
   }
-  __device__ __forceinline__ long long at(int64_t j) const {
-    return weight(Elem<T>::to_f(p[j]), q ? Elem<T>::to_f(q[j]) : 0.f, j);
+  __device__ __forceinline__ long long at(int j) const {
+    uint32_t h = 0, l = 0;
+    add(__saturatef(__fsub_rn(Elem<T>::to_f(p[j]), q ? Elem<T>::to_f(q[j]) : 0.f)), h, l);
+    return j == hit ? 0ll : ((long long)(h - kBias) << 20) + (l - kBias);
   }
-  // Sum over [begin, end), lane-strided, several loads in flight.
-  __device__ __forceinline__ long long sum(int64_t begin, int64_t end, int lane) const {
-    long long s = 0;
-    int64_t j = begin + lane;
-    for (; j + 7 * 32 < end; j += 8 * 32) {
-      float a[8], b[8];
+  // Sum over the 256 entries from j0 by one warp (those below V), every lane's.
+  __device__ __forceinline__ long long sum256(int j0, int V, int lane) const {
+    float a[8];
+    if (j0 + 256 <= V) {
+      if (wide) {
+        constexpr int N = Chunk<T>::N, U = 8 / N;
+        uint4 x[U], y[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = Elem<T>::to_f(p[j + 32 * i]);
+        for (int i = 0; i < U; ++i)
+          x[i] = __ldg(reinterpret_cast<const uint4*>(p + j0) + i * 32 + lane);
+        if (q) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) b[i] = q ? Elem<T>::to_f(q[j + 32 * i]) : 0.f;
+          for (int i = 0; i < U; ++i)
+            y[i] = __ldg(reinterpret_cast<const uint4*>(q + j0) + i * 32 + lane);
+        }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += weight(a[i], b[i], j + 32 * i);
+        for (int i = 0; i < U; ++i) Chunk<T>::to_f(x[i], a + i * N);
+        if (q) {
+          float b[8];
+#pragma unroll
+          for (int i = 0; i < U; ++i) Chunk<T>::to_f(y[i], b + i * N);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a[i] = __fsub_rn(a[i], b[i]);
+        }
+      } else {
+        const T* pr = p + j0 + lane;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = Elem<T>::to_f(__ldg(pr + 32 * i));
+        if (q) {
+          const T* qr = q + j0 + lane;
+          float b[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b[i] = Elem<T>::to_f(__ldg(qr + 32 * i));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a[i] = __fsub_rn(a[i], b[i]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + lane + 32 * i;
+        a[i] = 0.f;
+        if (j < V) a[i] = __fsub_rn(Elem<T>::to_f(p[j]), q ? Elem<T>::to_f(q[j]) : 0.f);
+      }
     }
-    for (; j < end; j += 32) s += at(j);
+    uint32_t h = 0, l = 0;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int i = 0; i < 8; ++i) add(__saturatef(a[i]), h, l);
+    // 256 parts of at most 2^20 each: the 32-bit sums wrap only by the biases
+    h = __reduce_add_sync(0xffffffffu, h - 8 * kBias);
+    l = __reduce_add_sync(0xffffffffu, l - 8 * kBias);
+    long long s = ((long long)h << 20) + l;
+    if ((unsigned)(hit - j0) < 256u) {  // the entry that is taken out (without q)
+      h = l = 0;
+      add(__saturatef(Elem<T>::to_f(p[hit])), h, l);
+      s -= ((long long)(h - kBias) << 20) + (l - kBias);
+    }
     return s;
   }
 };
 
-// The part (of `n` sums) that holds `level`, and the sum of those before it.
-__device__ __forceinline__ int verify_part(const long long* sums, int n, long long level,
-                                           long long* before) {
-  long long run = 0;
-  for (int i = 0; i < n; ++i) {
-    if (run + sums[i] > level) {
-      *before = run;
-      return i;
-    }
-    run += sums[i];
+__device__ __forceinline__ long long warp_scan(long long x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
-  *before = run;
-  return n - 1;
+  return x;
+}
+// By one warp: the first of `n` <= 32 PER sums whose running sum is above
+// `level` (some sum is), and the running sum before it. PER: sums per lane.
+template <int PER>
+__device__ __forceinline__ int verify_part(const long long* sums, int n, long long level, int lane,
+                                           long long* before) {
+  long long v[PER], mine = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    v[i] = lane * PER + i < n ? sums[lane * PER + i] : 0ll;
+    mine += v[i];
+  }
+  long long run = warp_scan(mine, lane);
+  const int f = __ffs(__ballot_sync(0xffffffffu, run > level)) - 1;
+  run -= mine;  // before this lane's
+  int at = 0;
+#pragma unroll
+  for (int i = 0; i + 1 < PER; ++i)
+    if (at == i && run + v[i] <= level) {
+      run += v[i];
+      ++at;
+    }
+  *before = __shfl_sync(0xffffffffu, run, f);
+  return f * PER + __shfl_sync(0xffffffffu, at, f);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyParams p) {
+  constexpr int NT = kVerifyThreads, kWarps = NT / 32;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  __shared__ long long sums[kVerifyWarps];
-  __shared__ long long all[kVerifyMaxCluster * kVerifyWarps];
-  __shared__ int s_accepted, s_n;
-  __shared__ int64_t s_hit;
+  __shared__ long long totals[2][kVerifyMaxCluster];
+  __shared__ long long sums[kVerifyBlocks];
+  __shared__ int s_accepted, s_n, s_hit;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int b = blockIdx.x / C;
+  const int b = blockIdx.x / C, V = (int)p.V;
+  // every CTA of the cluster runs before any of them writes into another
+  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
   grid_dependency_wait();
   launch_dependents();
 
   if (warp == 0) {
     int n = p.draft_lengths ? __ldg(p.draft_lengths + b) : p.T;
-    if (n < 0 || n > p.T) {
-      raise_error(0x2u);
-      n = n < 0 ? 0 : p.T;
-    }
-    int accepted = 0;
-    int64_t hit = -1;
-    for (int i0 = 0; i0 < n; i0 += 32) {
+    int accepted = 0, hit = -1;
+    for (int i0 = 0; i0 < p.T; i0 += 32) {
+      // drafts past n are read too (and not used), so that no read waits for n
       const int i = i0 + lane;
-      bool ok = i < n;
+      const bool in = i < p.T;
+      float u = 0.f, pt = 0.f, qt = 1.f;
       int64_t x = -1;
-      if (ok) {
+      if (in) {
+        u = p.accept_uniforms[(int64_t)b * p.T + i];
         x = p.draft_tokens[(int64_t)b * p.T + i];
-        ok = x >= 0 && x < p.V;
-        if (!ok) raise_error(0x40u);
       }
-      if (ok) {
-        const float pt = Elem<T>::to_f(
-            static_cast<const T*>(p.target)[((int64_t)b * (p.T + 1) + i) * p.V + x]);
-        const float qt =
-            p.draft ? Elem<T>::to_f(static_cast<const T*>(p.draft)[((int64_t)b * p.T + i) * p.V + x])
-                    : 1.f;
-        ok = __fmul_rn(p.accept_uniforms[(int64_t)b * p.T + i], qt) < pt;
+      const bool known = x >= 0 && x < V;
+      if (known) {
+        pt = Elem<T>::to_f(static_cast<const T*>(p.target)[((int64_t)b * (p.T + 1) + i) * V + x]);
+        if (p.draft)
+          qt = Elem<T>::to_f(static_cast<const T*>(p.draft)[((int64_t)b * p.T + i) * V + x]);
       }
-      const unsigned bad = __ballot_sync(0xffffffffu, i < n && !ok);
-      const int here = bad ? __ffs(bad) - 1 : (n - i0 < 32 ? n - i0 : 32);
+      if (i0 == 0 && (n < 0 || n > p.T)) {
+        raise_error(0x2u);
+        n = n < 0 ? 0 : p.T;
+      }
+      const unsigned bad =
+          __ballot_sync(0xffffffffu, i < n && !(known && __fmul_rn(u, qt) < pt));
+      const int left = n - i0 < 0 ? 0 : n - i0 < 32 ? n - i0 : 32;
+      const int here = bad ? __ffs(bad) - 1 : left;
+      if (i < n && lane <= here && !known) raise_error(0x40u);
       accepted += here;
-      if (bad) {
-        hit = __shfl_sync(0xffffffffu, x, here);
-        break;
-      }
+      if (bad) hit = __shfl_sync(0xffffffffu, known ? (int)x : -1, here);
+      if (bad || left < 32) break;
     }
     if (lane == 0) {
       s_accepted = accepted;
@@ -146,75 +218,96 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
       s_hit = hit;
     }
   }
+  const float u = __ldg(p.sample_uniforms + b);
   __syncthreads();
   const int accepted = s_accepted;
   const bool rejected = accepted < s_n;
   VerifyRow<T> row;
-  row.p = static_cast<const T*>(p.target) + ((int64_t)b * (p.T + 1) + accepted) * p.V;
+  row.p = static_cast<const T*>(p.target) + ((int64_t)b * (p.T + 1) + accepted) * V;
   row.q = rejected && p.draft
-              ? static_cast<const T*>(p.draft) + ((int64_t)b * p.T + accepted) * p.V
+              ? static_cast<const T*>(p.draft) + ((int64_t)b * p.T + accepted) * V
               : nullptr;
   row.hit = rejected && !p.draft ? s_hit : -1;
+  row.wide = ((reinterpret_cast<uintptr_t>(row.p) | reinterpret_cast<uintptr_t>(row.q)) & 15u) == 0;
 
-  const int parts = C * kVerifyWarps;
-  const int64_t seg = (p.V + parts - 1) / parts;
-  long long total = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    const int64_t lo = (int64_t)(rank * kVerifyWarps + warp) * seg;
-    const int64_t hi = lo + seg < p.V ? lo + seg : p.V;
-    const long long s = row.sum(lo < p.V ? lo : p.V, hi, lane);
-    if (lane == 0) sums[warp] = s;
-    cluster.sync();
-    if (tid < parts)
-      all[tid] = cluster.map_shared_rank(sums, tid / kVerifyWarps)[tid % kVerifyWarps];
-    cluster.sync();  // every remote read is done: a CTA may rewrite its sums or end
-    total = 0;
-    for (int i = 0; i < parts; ++i) total += all[i];
-    if (total > 0) break;
+  // this CTA's range: `blocks` blocks of `size` entries
+  const int share = (V + C - 1) / C;
+  const int size = 256 * ((share + 256 * kVerifyBlocks - 1) / (256 * kVerifyBlocks));
+  const int blocks = (share + size - 1) / size, first = rank * blocks * size;
+  constexpr int PER = kVerifyBlocks / 32;
+  long long total = 0, before = 0;
+  int pass = 0;
+  for (;; ++pass) {
+#pragma unroll 2
+    for (int x = warp; x < blocks; x += kWarps) {
+      long long s = 0;
+      for (int j = first + x * size; j < first + (x + 1) * size && j < V; j += 256)
+        s += row.sum256(j, V, lane);
+      if (lane == 0) sums[x] = s;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      long long mine = 0;
+      for (int i = lane; i < blocks; i += 32) mine += sums[i];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      if (C == 1) {
+        if (lane == 0) totals[pass][0] = mine;
+      }
+      if (C > 1) {
+        if (pass == 0) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        if (lane < C) cluster.map_shared_rank(&totals[pass][0], lane)[rank] = mine;
+      }
+    } else if (C > 1 && pass == 0) {
+      asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    }
+    if (C == 1) __syncthreads();
+    else cluster.sync();
+    total = before = 0;
+    for (int i = 0; i < C; ++i) {
+      if (i < rank) before += totals[pass][i];
+      total += totals[pass][i];
+    }
+    if (total > 0 || pass == 1) break;
     row.q = nullptr;  // no weight left after the difference: the target's own
     row.hit = -1;
+    row.wide = (reinterpret_cast<uintptr_t>(row.p) & 15u) == 0;
   }
   long long level = 0;
-  const float u = __ldg(p.sample_uniforms + b);
   if (u > 0.f) level = (long long)((double)total * (double)fminf(u, 1.f));
   if (level > total - 1) level = total - 1;
   if (level < 0) level = 0;
-  long long before;
-  const int part = total > 0 ? verify_part(all, parts, level, &before) : 0;
-  if (part / kVerifyWarps != rank) return;
+  // the CTA that holds the level (without any weight: the first)
+  if (total > 0 ? (level < before || level >= before + totals[pass][rank]) : rank != 0) return;
   int64_t* out = p.tokens + (int64_t)b * (p.T + 1);
-  for (int i = tid; i <= p.T; i += kVerifyThreads)
-    if (i != accepted) out[i] = i < accepted ? p.draft_tokens[(int64_t)b * p.T + i] : -1;
-  if (tid == 0) p.counts[b] = accepted + 1;
+  if (warp != 0) {
+    for (int i = tid - 32; i <= p.T; i += NT - 32)
+      if (i != accepted) out[i] = i < accepted ? p.draft_tokens[(int64_t)b * p.T + i] : -1;
+    if (tid == 32) p.counts[b] = accepted + 1;
+    return;
+  }
   if (total <= 0) {
-    if (tid == 0) out[accepted] = -1;
+    if (lane == 0) out[accepted] = -1;
     return;
   }
   level -= before;
-  // the segment, split over this CTA's warps
-  const int64_t s0 = (int64_t)part * seg, s1 = s0 + seg < p.V ? s0 + seg : p.V;
-  const int64_t sub = (s1 - s0 + kVerifyWarps - 1) / kVerifyWarps;
-  const int64_t lo = s0 + warp * sub < s1 ? s0 + warp * sub : s1, hi = lo + sub < s1 ? lo + sub : s1;
-  const long long s = row.sum(lo, hi, lane);
-  __syncthreads();
-  if (lane == 0) sums[warp] = s;
-  __syncthreads();
-  const int w = verify_part(sums, kVerifyWarps, level, &before);
-  if (w != warp) return;
+  const int x = verify_part<PER>(sums, blocks, level, lane, &before);
   level -= before;
-  for (int64_t j0 = lo; j0 < hi; j0 += 32) {
-    long long run = j0 + lane < hi ? row.at(j0 + lane) : 0ll;
+  const int lo = first + x * size, hi = lo + size < V ? lo + size : V;
+  for (int j0 = lo; j0 < hi; j0 += 256) {
+    long long w[8];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += y;
+    for (int i = 0; i < 8; ++i) w[i] = j0 + 32 * i + lane < hi ? row.at(j0 + 32 * i + lane) : 0ll;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const long long r = warp_scan(w[i], lane);
+      const unsigned above = __ballot_sync(0xffffffffu, r > level);
+      if (above) {
+        if (lane == 0) out[accepted] = j0 + 32 * i + (__ffs(above) - 1);
+        return;
+      }
+      level -= __shfl_sync(0xffffffffu, r, 31);
     }
-    const unsigned above = __ballot_sync(0xffffffffu, run > level);
-    if (above) {
-      if (lane == 0) out[accepted] = j0 + (__ffs(above) - 1);
-      return;
-    }
-    level -= __shfl_sync(0xffffffffu, run, 31);
   }
 }
 

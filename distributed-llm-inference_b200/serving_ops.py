@@ -16,14 +16,22 @@ import functools
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _DeviceGuard, _check, _stream_ptr, workspace
+from .ops import _DTYPES, _DeviceGuard, _stream_ptr, workspace
 
 
-def _check_same_device(first: torch.Tensor, *others) -> None:
-    for t in (first, *others):
+def _refuse(message: str):
+    raise RuntimeError(message)
+
+
+# The checks below are plain conditions, and a tensor's properties are read once: a
+# call of a few microseconds on the GPU should not wait for its arguments' checks.
+def _check_same_device(device: int, *tensors) -> None:
+    for t in tensors:
         if t is not None:
-            _check(t.device == first.device, "all tensors must be on the same GPU")
-            _check(t.is_contiguous(), "all tensors must be contiguous")
+            if t.get_device() != device:
+                _refuse("all tensors must be on the same GPU")
+            if not t.is_contiguous():
+                _refuse("all tensors must be contiguous")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -56,60 +64,77 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     head: into ``scores_out`` (default: in place). Returns (out, scores) then.
     Asynchronous on the current stream; `impl` pins the kernels.
     """
-    _check(q.is_cuda, "query must be on CUDA")
-    _check_same_device(q, k, v, prefix_table, tables, lengths, counts, scores, scores_out)
-    _check(q.dim() in (3, 4) and k.dim() == 4 and k.shape == v.shape, "invalid Q/K/V shapes")
-    if q.dim() == 4:
-        B, T, H, D = q.shape
+    device = q.get_device()
+    if device < 0:
+        _refuse("query must be on CUDA")
+    _check_same_device(device, q, k, v, prefix_table, tables, lengths, counts, scores, scores_out)
+    q_shape, k_shape = q.shape, k.shape
+    if len(k_shape) != 4 or v.shape != k_shape:
+        _refuse("invalid Q/K/V shapes")
+    if len(q_shape) == 4:
+        B, T, H, D = q_shape
+    elif len(q_shape) == 3:
+        (B, H, D), T = q_shape, 1
     else:
-        (B, H, D), T = q.shape, 1
-    N, bs, KVH, Dk = k.shape
-    _check(B > 0 and T > 0 and H > 0 and 0 < D <= 256, "invalid query shape")
-    _check(N > 0 and bs > 0 and KVH > 0 and Dk == D, "invalid cache shape")
-    _check(H % KVH == 0, "query heads must be a multiple of KV heads")
-    _check(q.dtype in _DTYPES, "use FP32 or FP16")
-    _check(k.dtype == q.dtype and v.dtype == q.dtype, "dtype mismatch")
-    _check(tables.dtype == torch.int32 and lengths.dtype == torch.int32
-           and prefix_table.dtype == torch.int32, "metadata must be int32")
-    _check(tables.dim() == 2 and tables.size(0) == B and prefix_table.dim() == 1,
-           "invalid block tables")
-    _check(lengths.dim() == 1 and lengths.size(0) == B, "invalid lengths")
-    if counts is not None:
-        _check(counts.dtype == torch.int32 and counts.shape == (B,), "invalid token counts")
+        _refuse("invalid Q/K/V shapes")
+    N, bs, KVH, Dk = k_shape
+    if not (B > 0 and T > 0 and H > 0 and 0 < D <= 256):
+        _refuse("invalid query shape")
+    if not (N > 0 and bs > 0 and KVH > 0 and Dk == D):
+        _refuse("invalid cache shape")
+    if H % KVH:
+        _refuse("query heads must be a multiple of KV heads")
+    dtype = q.dtype
+    dt = _DTYPES.get(dtype)
+    if dt is None:
+        _refuse("use FP32 or FP16")
+    if k.dtype != dtype or v.dtype != dtype:
+        _refuse("dtype mismatch")
+    if not (tables.dtype == lengths.dtype == prefix_table.dtype == torch.int32):
+        _refuse("metadata must be int32")
+    if tables.dim() != 2 or tables.shape[0] != B or prefix_table.dim() != 1:
+        _refuse("invalid block tables")
+    if lengths.shape != (B,):
+        _refuse("invalid lengths")
+    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (B,)):
+        _refuse("invalid token counts")
     prefix_length, max_length = int(prefix_length), int(max_length)
-    _check(0 <= prefix_length <= prefix_table.size(0) * bs, "invalid prefix length")
-    _check(0 <= max_length <= tables.size(1) * bs, "invalid context bound")
-    width = 0
+    pages, table_width = prefix_table.shape[0], tables.shape[1]
+    if not 0 <= prefix_length <= pages * bs:
+        _refuse("invalid prefix length")
+    if not 0 <= max_length <= table_width * bs:
+        _refuse("invalid context bound")
+    width, scores_ptr, scores_out_ptr = 0, None, None
     if scores is not None:
-        _check(scores.dtype == torch.float32 and scores.dim() == 3
-               and scores.shape[:2] == (B, KVH), "scores must be fp32 [batch, kv_heads, tokens]")
-        width = scores.size(2)
-        _check(width >= max_length, "scores must hold max_length tokens")
+        if scores.dtype != torch.float32 or scores.dim() != 3 or scores.shape[:2] != (B, KVH):
+            _refuse("scores must be fp32 [batch, kv_heads, tokens]")
+        width = scores.shape[2]
+        if width < max_length:
+            _refuse("scores must hold max_length tokens")
         if scores_out is None:
             scores_out = scores
-        _check(scores_out.shape == scores.shape and scores_out.dtype == torch.float32,
-               "invalid scores output")
-    else:
-        _check(scores_out is None, "scores_out needs scores")
+        elif scores_out.shape != scores.shape or scores_out.dtype != torch.float32:
+            _refuse("invalid scores output")
+        if width:
+            scores_ptr, scores_out_ptr = scores.data_ptr(), scores_out.data_ptr()
+    elif scores_out is not None:
+        _refuse("scores_out needs scores")
     if out is None:
         out = torch.empty_like(q)
-    else:
-        _check(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()
-               and out.device == q.device, "invalid output tensor")
-    lib, dt = _lib.load(), _DTYPES[q.dtype]
+    elif not (out.shape == q_shape and out.dtype == dtype and out.is_contiguous()
+              and out.get_device() == device):
+        _refuse("invalid output tensor")
     with _DeviceGuard(q.device):
         stream = _stream_ptr(q.device)
-        need = _prefix_workspace(q.device.index, B, T, H, KVH, D, prefix_length, max_length, dt,
-                                 scores is not None)
+        need = _prefix_workspace(device, B, T, H, KVH, D, prefix_length, max_length, dt,
+                                 width > 0)
         ws = workspace(q.device, stream, need, "shared_prefix")
-        rc = lib.pdb_shared_prefix_attention_impl(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), prefix_table.data_ptr(),
-            prefix_table.size(0), prefix_length, tables.data_ptr(), lengths.data_ptr(),
-            counts.data_ptr() if counts is not None else None,
-            scores.data_ptr() if width else None, scores_out.data_ptr() if width else None, width,
-            out.data_ptr(), B, T, H, D, N, bs, KVH, tables.size(1), max_length, dt,
-            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-            stream, int(impl))
+        rc = _lib.load().pdb_shared_prefix_attention_impl(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), prefix_table.data_ptr(), pages,
+            prefix_length, tables.data_ptr(), lengths.data_ptr(),
+            counts.data_ptr() if counts is not None else None, scores_ptr, scores_out_ptr, width,
+            out.data_ptr(), B, T, H, D, N, bs, KVH, table_width, max_length, dt,
+            ws.data_ptr() if ws is not None else None, need, stream, impl)
     _lib.check(rc, "shared_prefix_attention")
     return out if scores is None else (out, scores_out)
 
@@ -132,35 +157,44 @@ def verify_drafts(draft_tokens: torch.Tensor, target_probs: torch.Tensor,
     of 2^-40), so equal inputs give equal tokens on any GPU; a row without any
     weight gives -1.
     """
-    _check(target_probs.is_cuda, "probabilities must be on CUDA")
-    _check_same_device(target_probs, draft_tokens, accept_uniforms, sample_uniforms, draft_probs,
-                       draft_lengths)
-    _check(draft_tokens.dim() == 2 and target_probs.dim() == 3, "invalid probabilities shape")
-    B, T = draft_tokens.shape
-    V = target_probs.size(2)
-    _check(B > 0 and T > 0 and V > 0 and target_probs.shape == (B, T + 1, V),
-           "invalid probabilities shape")
-    _check(target_probs.dtype in _DTYPES, "use FP32 or FP16")
+    device = target_probs.get_device()
+    if device < 0:
+        _refuse("probabilities must be on CUDA")
+    _check_same_device(device, target_probs, draft_tokens, accept_uniforms, sample_uniforms,
+                       draft_probs, draft_lengths)
+    shape = target_probs.shape
+    if draft_tokens.dim() != 2 or len(shape) != 3:
+        _refuse("invalid probabilities shape")
+    (B, T), V = draft_tokens.shape, shape[2]
+    if not (B > 0 and T > 0 and V > 0 and shape[0] == B and shape[1] == T + 1):
+        _refuse("invalid probabilities shape")
+    dtype = target_probs.dtype
+    dt = _DTYPES.get(dtype)
+    if dt is None:
+        _refuse("use FP32 or FP16")
     if draft_probs is not None:
-        _check(draft_probs.shape == (B, T, V), "invalid probabilities shape")
-        _check(draft_probs.dtype == target_probs.dtype, "dtype mismatch")
-    _check(draft_tokens.dtype == torch.int64, "draft tokens must be int64")
-    _check(accept_uniforms.dtype == torch.float32 and accept_uniforms.shape == (B, T)
-           and sample_uniforms.dtype == torch.float32 and sample_uniforms.shape == (B,),
-           "invalid random numbers")
-    if draft_lengths is not None:
-        _check(draft_lengths.dtype == torch.int32 and draft_lengths.shape == (B,),
-               "invalid draft lengths")
-    tokens = torch.empty((B, T + 1), dtype=torch.int64, device=target_probs.device)
-    counts = torch.empty((B,), dtype=torch.int32, device=target_probs.device)
+        if draft_probs.shape != (B, T, V):
+            _refuse("invalid probabilities shape")
+        if draft_probs.dtype != dtype:
+            _refuse("dtype mismatch")
+    if draft_tokens.dtype != torch.int64:
+        _refuse("draft tokens must be int64")
+    if not (accept_uniforms.dtype == sample_uniforms.dtype == torch.float32
+            and accept_uniforms.shape == (B, T) and sample_uniforms.shape == (B,)):
+        _refuse("invalid random numbers")
+    if draft_lengths is not None and (draft_lengths.dtype != torch.int32
+                                      or draft_lengths.shape != (B,)):
+        _refuse("invalid draft lengths")
+    tokens = draft_tokens.new_empty((B, T + 1))
+    counts = (torch.empty_like(draft_lengths) if draft_lengths is not None
+              else draft_tokens.new_empty((B,), dtype=torch.int32))
     with _DeviceGuard(target_probs.device):
         rc = _lib.load().pdb_verify_drafts(
             draft_tokens.data_ptr(), target_probs.data_ptr(),
             draft_probs.data_ptr() if draft_probs is not None else None,
             accept_uniforms.data_ptr(), sample_uniforms.data_ptr(),
             draft_lengths.data_ptr() if draft_lengths is not None else None, tokens.data_ptr(),
-            counts.data_ptr(), B, T, V, _DTYPES[target_probs.dtype],
-            _stream_ptr(target_probs.device))
+            counts.data_ptr(), B, T, V, dt, _stream_ptr(target_probs.device))
     _lib.check(rc, "verify_drafts")
     return tokens, counts
 
@@ -179,35 +213,47 @@ def evict_tokens(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor, tables:
     layer and head). Returns (kept int32 [B, KVH, budget]: indices, then -1;
     new_lengths int32 [B]; new_scores like scores, 0 past the kept tokens).
     """
-    _check(k.is_cuda, "cache must be on CUDA")
-    _check_same_device(k, v, scores, tables, lengths, new_tables)
-    _check(k.dim() == 4 and k.shape == v.shape and k.numel() > 0, "invalid cache shape")
-    _check(k.dtype in _DTYPES, "use FP32 or FP16")
-    _check(v.dtype == k.dtype, "dtype mismatch")
-    N, bs, KVH, D = k.shape
-    _check(lengths.dim() == 1 and lengths.size(0) > 0, "invalid lengths")
-    B = lengths.size(0)
-    _check(scores.dtype == torch.float32 and scores.dim() == 3 and scores.shape[:2] == (B, KVH)
-           and scores.size(2) > 0, "scores must be fp32 [batch, kv_heads, tokens]")
-    _check(tables.dtype == torch.int32 and lengths.dtype == torch.int32
-           and new_tables.dtype == torch.int32, "metadata must be int32")
-    _check(tables.dim() == 2 and tables.size(0) == B and tables.size(1) > 0
-           and new_tables.dim() == 2 and new_tables.size(0) == B and new_tables.size(1) > 0,
-           "invalid block tables")
-    budget, recent = int(budget), int(recent)
-    _check(budget > 0, "invalid budget")
-    _check(0 <= recent <= budget, "recent tokens must fit the budget")
-    S = scores.size(2)
-    _check(new_tables.size(1) * bs >= min(budget, S, tables.size(1) * bs),
-           "new tables must hold the budget")
-    kept = torch.empty((B, KVH, budget), dtype=torch.int32, device=k.device)
+    device = k.get_device()
+    if device < 0:
+        _refuse("cache must be on CUDA")
+    _check_same_device(device, k, v, scores, tables, lengths, new_tables)
+    k_shape = k.shape
+    if len(k_shape) != 4 or v.shape != k_shape or 0 in k_shape:
+        _refuse("invalid cache shape")
+    dt = _DTYPES.get(k.dtype)
+    if dt is None:
+        _refuse("use FP32 or FP16")
+    if v.dtype != k.dtype:
+        _refuse("dtype mismatch")
+    N, bs, KVH, D = k_shape
+    if lengths.dim() != 1 or lengths.shape[0] == 0:
+        _refuse("invalid lengths")
+    B = lengths.shape[0]
+    s_shape = scores.shape
+    if not (scores.dtype == torch.float32 and len(s_shape) == 3 and s_shape[0] == B
+            and s_shape[1] == KVH and s_shape[2] > 0):
+        _refuse("scores must be fp32 [batch, kv_heads, tokens]")
+    if not (tables.dtype == lengths.dtype == new_tables.dtype == torch.int32):
+        _refuse("metadata must be int32")
+    t_shape, n_shape = tables.shape, new_tables.shape
+    if not (len(t_shape) == 2 and t_shape[0] == B and t_shape[1] > 0
+            and len(n_shape) == 2 and n_shape[0] == B and n_shape[1] > 0):
+        _refuse("invalid block tables")
+    budget, recent, S = int(budget), int(recent), s_shape[2]
+    if budget <= 0:
+        _refuse("invalid budget")
+    if not 0 <= recent <= budget:
+        _refuse("recent tokens must fit the budget")
+    if n_shape[1] * bs < min(budget, S, t_shape[1] * bs):
+        _refuse("new tables must hold the budget")
+    kept = lengths.new_empty((B, KVH, budget))
     new_lengths = torch.empty_like(lengths)
     new_scores = torch.empty_like(scores)
     with _DeviceGuard(k.device):
         rc = _lib.load().pdb_evict_tokens(
             k.data_ptr(), v.data_ptr(), scores.data_ptr(), S, tables.data_ptr(),
             lengths.data_ptr(), new_tables.data_ptr(), kept.data_ptr(), new_lengths.data_ptr(),
-            new_scores.data_ptr(), B, D, N, bs, KVH, tables.size(1), new_tables.size(1), budget,
-            recent, _DTYPES[k.dtype], _stream_ptr(k.device))
+            new_scores.data_ptr(), B, D, N, bs, KVH, t_shape[1], n_shape[1], budget, recent, dt,
+            _stream_ptr(k.device))
     _lib.check(rc, "evict_tokens")
     return kept, new_lengths, new_scores
