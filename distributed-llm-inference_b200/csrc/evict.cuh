@@ -106,7 +106,7 @@ __device__ __forceinline__ int evict_scan_counts(int* counts) {
 // Candidates per round of the CTA: E stripes of one per thread.
 constexpr int kEvictWideBits = 12, kEvictList = 2048;
 template <int E>
-__global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kEvictThreads, 3) evict_select_kernel(const EvictParams p) {
   __shared__ int red[2 * kEvictWarps];
   __shared__ int tie_counts[16 * E + 1], keep_counts[16 * E + 1], list_n;
   __shared__ uint32_t list[kEvictList];
@@ -217,24 +217,32 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ev
   const unsigned below = (1u << lane) - 1;
   for (int base = 0; base < cand; base += ROUND) {
     if (!one) load(base);
-    unsigned eq[E], keep[E];
+    // ballots are taken again where they are needed: kept, they would cost 32
+    // registers and the third CTA per SM
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      eq[e] = __ballot_sync(0xffffffffu, key[e] == thr && key[e] != 0u);
-      if (lane == 0) tie_counts[e * kEvictWarps + warp] = __popc(eq[e]);
+      const unsigned eq = __ballot_sync(0xffffffffu, key[e] == thr && key[e] != 0u);
+      if (lane == 0) tie_counts[e * kEvictWarps + warp] = __popc(eq);
     }
     const int tie_sum = evict_scan_counts<E>(tie_counts);
+    unsigned mine = 0;  // bit e: this thread's key of stripe e stays
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int rank = tie_base + tie_counts[e * kEvictWarps + warp] + __popc(eq[e] & below);
-      keep[e] = __ballot_sync(0xffffffffu, key[e] > thr || ((eq[e] >> lane & 1u) && rank < ties));
-      if (lane == 0) keep_counts[e * kEvictWarps + warp] = __popc(keep[e]);
+      const bool tie = key[e] == thr && key[e] != 0u;
+      const unsigned eq = __ballot_sync(0xffffffffu, tie);
+      const int rank = tie_base + tie_counts[e * kEvictWarps + warp] + __popc(eq & below);
+      const bool stays = key[e] > thr || (tie && rank < ties);
+      mine |= (unsigned)stays << e;
+      const unsigned keep = __ballot_sync(0xffffffffu, stays);
+      if (lane == 0) keep_counts[e * kEvictWarps + warp] = __popc(keep);
     }
     const int keep_sum = evict_scan_counts<E>(keep_counts);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (keep[e] >> lane & 1u) {
-        const int at = out_base + keep_counts[e * kEvictWarps + warp] + __popc(keep[e] & below);
+      const bool stays = mine >> e & 1u;
+      const unsigned keep = __ballot_sync(0xffffffffu, stays);
+      if (stays) {
+        const int at = out_base + keep_counts[e * kEvictWarps + warp] + __popc(keep & below);
         const int j = base + e * kEvictThreads + tid;
         kept[at] = j;
         nsc[at] = __ldg(sc + j);

@@ -181,8 +181,9 @@ cudaError_t launch_prefix_simt(int dev, const pdb::PrefixParams& p, bool prefix,
   const int own_tiles = prefix ? 0 : (int)((TG + RT - 1) / RT);
   const int64_t gx = prefix ? (int64_t)prefix_tiles * p.prefix.slots
                             : (int64_t)p.B * own_tiles * p.own.slots;
+  const int wide = p.D % 4 == 0 && aligned16(p.k_pool) && aligned16(p.v_pool);
   return launch_pdl(fn, dim3((unsigned)gx, (unsigned)p.KVH), dim3(C::NT), C::SMEM, st, p,
-                    prefix_tiles, own_tiles);
+                    prefix_tiles, own_tiles, wide);
 }
 template <typename T, int DP>
 cudaError_t launch_prefix_simt_rows(int dev, const pdb::PrefixParams& p, bool prefix,
@@ -221,7 +222,7 @@ cudaError_t launch_spans_mma(int dev, const pdb::PrefixParams& p, const PrefixPl
   ss.nseq = pl.own_kernel == kSpanMma ? p.B : 0;
   ss.part = ss.nseq ? p.own : p.prefix;
   ss.prefix_segments = ss.has_prefix ? p.prefix.segments : 0;
-  ss.beside = pl.prefix_kernel == kSpanTc;
+  ss.beside = p.beside;
   const int nt = pl.nt, grid = ss.part.grid;
   if (p.D == 64) {
     if (nt == 1) return launch_span_mma<64, 1, 1>(dev, p, ss, grid, st, kmap, vmap);
@@ -409,6 +410,7 @@ int pdb_shared_prefix_attention_impl(
   p.table_width = (int)table_width;
   p.prefix_length = (int)prefix_length; p.max_length = (int)max_length;
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
+  p.beside = (pl.prefix_kernel == kSpanTc || pl.prefix_kernel == kSpanSimt) && pl.own_kernel;
   CUtensorMap kmap, vmap, kunits, vunits;  // boxes of the tcgen05 kernel, of the mma.sync kernel
   const bool tc = pl.prefix_kernel == kSpanTc;
   const bool mma = pl.prefix_kernel == kSpanMma || pl.own_kernel == kSpanMma;
