@@ -23,7 +23,8 @@ enum SpanKernel { kSpanNone = 0, kSpanSimt, kSpanMma, kSpanTc };
 
 struct PrefixPlan {
   int prefix_kernel, own_kernel;
-  int nt;  // kSpanMma: 8-row tiles per segment
+  int nt;      // kSpanMma: 8-row tiles per segment
+  int splits;  // kSpanTc: ranges per item, or 0
   pdb::PartSet prefix, own;
   size_t prefix_ml, prefix_o, prefix_dir, own_ml, own_o, own_dir, lse_off, logits_off, total;
 };
@@ -53,27 +54,30 @@ constexpr int kSpanCtasPerSm = 2;
 // below, it is one more key set of the mma.sync kernel's launch.
 constexpr int64_t kTcRows = 33;
 
-// SMs of the tcgen05 kernel when the mma.sync kernel runs beside it on the others:
-// the split with the earlier end by the measured rates (a unit of 256 rows x 128
-// keys takes an SM 2.3 us; 64 keys of own context its share of HBM, 0.74 us per 32
-// KB, and not less than 0.5; about 10 and 8 us pass before and after), or all SMs
-// one after the other where that ends no later. Own lengths are on the device:
-// half the bound is taken. (B200, one token for 64 sequences, prefix 4096: 67 us on
-// all SMs in turn, 43.5 with 40 SMs for the prefix; 20 rows of four times the
-// lengths: no difference.)
-int tc_sms(int sms, double tc_units, double own_units, int64_t D) {
-  const double tc = 2.3 * tc_units, own = own_units * (D == 128 ? 0.74 : 0.5);
-  const double in_turn = 10 + tc / sms + 6 + own / sms;
-  double best = in_turn;
-  int n = 0;
-  for (int x = 1; x < sms; ++x) {
-    const double a = 10 + tc / x, b = 8 + own / (sms - x), t = a > b ? a : b;
-    if (t < 0.95 * in_turn && t < best) {
-      best = t;
-      n = x;
+// Ranges per item of the tcgen05 kernel (items: query tile pairs of all kv heads, with
+// `tiles` key tiles each) when the mma.sync kernel runs beside it on the SMs that
+// are left: those with the earlier end by the measured rates (a key tile 1.9 us
+// after 10 us of start and end; own contexts 0.74 us of an SM's time per 64 keys of
+// head_dim 128, its share of HBM, 0.5 at 64, after 8 us), or 0 where one after the
+// other on all SMs ends no later. Own lengths are on the device: half the bound is
+// taken. (B200, one token for 64 sequences over a prefix of 4096: 57 us in turn, 37
+// with 32 SMs for the prefix, 49 with 24, 42 with 60; 256 x 4 tokens over 8192 with
+// own contexts to 2048: 356 us in turn, 390 with half of the SMs.)
+int tc_splits(int sms, int64_t items, int64_t tiles, double own_units, int64_t D) {
+  const double own = own_units * (D == 128 ? 0.74 : 0.5);
+  const int64_t all = sms / items < 1 ? 1 : sms / items;
+  const double tc_all = items * all <= sms ? (double)((tiles + all - 1) / all)
+                                           : (double)(items * tiles) / sms;
+  double best = 10 + 1.9 * tc_all + 12 + own / sms;
+  int splits = 0;
+  for (int64_t k = 1; k <= tiles && items * k < sms; ++k) {
+    const double a = 10 + 1.9 * ((tiles + k - 1) / k), b = 8 + own / (sms - items * k);
+    if ((a > b ? a : b) < best) {
+      best = a > b ? a : b;
+      splits = (int)k;
     }
   }
-  return n;  // 0: in turn
+  return splits;
 }
 
 PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, int64_t D, int64_t P,
@@ -104,15 +108,16 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
     s.R = 256;
     s.half = (int)(128 / G);
     s.segments = (int)((B * T + 2 * s.half - 1) / (2 * s.half));
-    const int64_t units = KVH * s.segments * ((P + 127) / 128);
-    int n = 0;
+    const int64_t items = KVH * s.segments, tiles = (P + 127) / 128;
     if (pl.own_kernel == kSpanMma) {
       const int64_t r = 8 * span_nt(TG);
-      n = tc_sms(sms, (double)units,
-                 (double)(B * KVH * ((TG + r - 1) / r)) * (max_length / 128.0 + 1), D);
+      pl.splits = tc_splits(sms, items, tiles,
+                            (double)(B * KVH * ((TG + r - 1) / r)) * (max_length / 128.0 + 0.3), D);
+      beside_sms = (int)items * pl.splits;
     }
-    beside_sms = n;
-    s.grid = (int)std::min<int64_t>(n ? n : sms, units);
+    if (!pl.splits && items <= sms / 2)  // on all SMs: whole ranges where items are few
+      pl.splits = (int)std::min<int64_t>(sms / items, tiles);
+    s.grid = (int)(pl.splits ? items * pl.splits : std::min<int64_t>(sms, items * tiles));
     prefix_parts = (size_t)(KVH * s.segments + s.grid) * s.R;
   }
   if (pl.own_kernel == kSpanSimt) {
@@ -263,7 +268,7 @@ bool encode_group_map(CUtensorMap* m, const void* q, int64_t R, int64_t heads, i
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 template <int D>
-cudaError_t launch_prefix_tc(int dev, const pdb::PrefixParams& p, cudaStream_t st,
+cudaError_t launch_prefix_tc(int dev, const pdb::PrefixParams& p, int splits, cudaStream_t st,
                              const CUtensorMap& kmap, const CUtensorMap& vmap) {
   using C = pdb::PrefixTc<D>;
   auto* fn = &pdb::prefix_tc_kernel<D>;
@@ -279,6 +284,7 @@ cudaError_t launch_prefix_tc(int dev, const pdb::PrefixParams& p, cudaStream_t s
   t.per_tile = p.prefix.half;
   t.pairs = p.prefix.segments;
   t.key_tiles = (p.prefix_length + C::BN - 1) / C::BN;
+  t.splits = splits;
   t.dir = p.prefix.dir;
   t.prefix_length = p.prefix_length;
   t.block_size = p.block_size; t.bs_shift = p.bs_shift;
@@ -421,8 +427,8 @@ int pdb_shared_prefix_attention_impl(
     return fail(PDB_ERR_CUDA, "cuTensorMapEncodeTiled failed for the KV pools");
   cudaError_t e = cudaSuccess;
   if (pl.prefix_kernel == kSpanTc)
-    e = head_dim == 64 ? launch_prefix_tc<64>(dev, p, st, kmap, vmap)
-                       : launch_prefix_tc<128>(dev, p, st, kmap, vmap);
+    e = head_dim == 64 ? launch_prefix_tc<64>(dev, p, pl.splits, st, kmap, vmap)
+                       : launch_prefix_tc<128>(dev, p, pl.splits, st, kmap, vmap);
   else if (pl.prefix_kernel == kSpanSimt)
     e = launch_spans_simt(dev, dtype, p, true, st);
   if (e == cudaSuccess && mma)

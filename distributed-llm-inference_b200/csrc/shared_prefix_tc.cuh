@@ -4,9 +4,11 @@
 // All B T G rows of a kv head see the whole prefix, so this is a dense product
 // pair per kv head: S = Q K^T, O = P V with M = B T G. An item is (kv head,
 // pair of 128-row query tiles); all items have the same number of 128-key
-// tiles, and the (item, key tile) units are cut into one contiguous range per
-// CTA of equal length: a CTA works on the end of one item and the start of the
-// next. CTA c's piece of item i is piece i + c of the partials.
+// tiles. With few items each is cut into `splits` ranges, one per CTA; else the
+// (item, key tile) units are cut into one contiguous range per CTA of equal
+// length, and a CTA works on the end of one item and the start of the next (a
+// second piece costs it a second set of queries and a second epilogue, 5 us). CTA
+// c's piece of item i is piece i + c of the partials.
 //
 // One CTA per SM, eleven warps:
 //   * warps 0-3 and 4-7: softmax of query tile 0 and 1, one row per thread: read
@@ -22,6 +24,10 @@
 //     The MMAs of a CTA run in issue order, so S_{j+1} may overwrite P_j
 //     without a barrier, and the commit that publishes S_{j+1} also says that
 //     O holds P_j V_j (what a rescale needs).
+// Measured on 4096 rows x 8192 keys x 8 heads: 1.14 PFLOP/s. 64-key tiles with two S
+// buffers per query tile, with one or two issuing warps, and two threads per row
+// were no faster (128 and 130 us against 120), two threads per row on 128-key
+// tiles slower (they spill).
 // TMEM: S0 S1 O0 O1, 128 columns each = all 512.
 // Query rows: a tile holds floor(128 / G) tokens with all G heads of the kv
 // head, one TMA box {64 columns, G heads, floor(128 / G) tokens}, so any group
@@ -45,6 +51,7 @@ struct PrefixTcParams {
   int per_tile;               // tokens per 128-row tile
   int pairs;                  // pairs of query tiles per kv head
   int key_tiles;              // 128-key tiles of the prefix
+  int splits;                 // ranges per item, or 0: equal ranges over all units
   int prefix_length, block_size, bs_shift;
   float scale_log2;
 };
@@ -157,7 +164,15 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
   // this CTA's units [u0, u1) of (item, key tile)
   const int units = p.KVH * p.pairs * p.key_tiles;
   const int ctas = unit_ctas(units, (int)gridDim.x), me = (int)blockIdx.x;
-  const int u0 = unit_begin(me, units, ctas), u1 = unit_begin(me + 1, units, ctas);
+  int u0, u1;
+  if (p.splits) {
+    const int it = me / p.splits, part = me - it * p.splits;
+    u0 = it * p.key_tiles + unit_begin(part, p.key_tiles, p.splits);
+    u1 = it * p.key_tiles + unit_begin(part + 1, p.key_tiles, p.splits);
+  } else {
+    u0 = unit_begin(me, units, ctas);
+    u1 = unit_begin(me + 1, units, ctas);
+  }
   // Piece that starts at unit u: item, first key tile, number of key tiles.
   auto piece = [&](int u, int& item, int& j0, int& nj) {
     item = u / p.key_tiles;
@@ -315,12 +330,16 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
       const int pair = item % p.pairs;
       if (i < tiles_of(pair)) {
         float m_used = -INFINITY, l = 0.f;
-        for (int j = 0; j < nj; ++j, ++tile) {
-          wait(&s_full[i], (uint32_t)tile & 1u);
+        // Round -1 of the first piece runs this code on what TMEM holds, while the
+        // first tiles are on their way, and throws the result away: it brings the
+        // code, whose first execution otherwise waits on instruction fetches.
+        for (int j = n == 0 ? -1 : 0; j < nj; ++j) {
+          const bool real = j >= 0;
+          if (real) wait(&s_full[i], (uint32_t)tile & 1u);
           tc_fence_after();
           // Pass 1: the row's maximum. The second half of the logits stays in
           // registers, the first is read again: 128 at once would not fit.
-          const int valid = p.prefix_length - (j0 + j) * BN;
+          const int valid = real ? p.prefix_length - (j0 + j) * BN : BN;
           uint32_t s[64];
           float top = -INFINITY;
 #pragma unroll
@@ -345,7 +364,7 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
           // logits are in registers by then.
           uint32_t pk[32];
           float sum = weights64(s, pk, c, ref);
-          tc_st32(s_col + 96, pk);
+          if (real) tc_st32(s_col + 96, pk);
           tc_ld32(s_col, s);
           tc_ld32(s_col + 32, s + 32);
           tc_wait_ld();
@@ -353,8 +372,13 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
           tc_reg_fence32(s + 32);
           mask64(s, valid);
           sum += weights64(s, pk, c, ref);
-          tc_st32(s_col + 64, pk);
           l = l * alpha + sum;
+          if (!real) {
+            m_used = -INFINITY;
+            l = 0.f;
+            continue;
+          }
+          tc_st32(s_col + 64, pk);
           if (valid < BN && i == 0) {
             // V rows past the prefix (stale cells of its last unit): zeros. K and V
             // alternate in the ring: this tile's V is buffer 2 * tile + 1.
@@ -385,6 +409,7 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[i]);
+          ++tile;
         }
         // the piece's partial: O rows through this warp's quarter of the query
         // buffer, 64 columns at a time, so that stores cover whole row segments
