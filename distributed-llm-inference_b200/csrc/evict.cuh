@@ -7,15 +7,15 @@
 // keeps its own tokens, as a page holds each head's row separately.
 //
 // evict_select_kernel: one CTA per (sequence, kv head). Scores become 32-bit
-// keys in the order of the floats; the threshold (the largest key that at
-// least m - r candidates reach) is found bit by bit from the top, counting the
-// candidates at or above a trial key, until a count is exact. The first
-// kEvictWideBits bits count keys in registers; the keys that share those bits
-// with the threshold are then gathered in shared memory and only they are counted
-// on (histograms instead serialise on the few bins that scores of like magnitude
-// share). Counts per stripe of 32 scores, scanned once, number the ties and the
-// kept tokens in index order. Bound by instruction issue: 48 x 8 heads of up to
-// 8192 scores took 53 us with every bit counted over every key at one CTA per SM.
+// keys in the order of the floats (on a scale that is roughly logarithmic, so that
+// scores of unlike magnitude spread evenly). The threshold is the largest key that
+// at least m - r candidates reach: a histogram of the keys over kEvictBins equal
+// steps of their range names the step that holds it, and the few keys of that step
+// are ranked against each other. (Where one step holds too many keys to rank, or to
+// list, the threshold's bits are found one by one, by counting. Counting alone, bit
+// by bit over all keys, took 53 us for 48 x 8 heads of up to 8192 scores, bits past
+// the twelfth over a list 34, this MEASURED.) Counts per stripe of 32 scores, scanned
+// once, number the ties and the kept tokens in index order.
 // evict_move_kernel: copies rows in 16-byte pieces; bound by HBM.
 #pragma once
 
@@ -104,12 +104,13 @@ __device__ __forceinline__ int evict_scan_counts(int* counts) {
 }
 
 // Candidates per round of the CTA: E stripes of one per thread.
-constexpr int kEvictWideBits = 12, kEvictList = 2048;
+constexpr int kEvictBins = 2048, kEvictList = 2048, kEvictRank = 512;
 template <int E>
 __global__ void __launch_bounds__(kEvictThreads, 3) evict_select_kernel(const EvictParams p) {
   __shared__ int red[2 * kEvictWarps];
-  __shared__ int tie_counts[16 * E + 1], keep_counts[16 * E + 1], list_n;
-  __shared__ uint32_t list[kEvictList];
+  __shared__ int tie_counts[16 * E + 1], keep_counts[16 * E + 1], list_n, s_bin, s_higher;
+  __shared__ uint32_t list[kEvictList], s_thr;
+  __shared__ int bins[kEvictBins];
   int turn = 0;
   const int bh = blockIdx.x, b = bh / p.KVH, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dependency_wait();
@@ -145,64 +146,112 @@ __global__ void __launch_bounds__(kEvictThreads, 3) evict_select_kernel(const Ev
   for (int64_t i = m + tid; i < p.S; i += kEvictThreads) nsc[i] = 0.f;
   for (int i = m + tid; i < p.budget; i += kEvictThreads) kept[i] = -1;
   uint32_t thr = 0u;  // the largest key that at least `want` candidates reach
-  if (want < cand) {  // want == cand keeps all: threshold 0
-    bool exact = false;
-    int bit = 31, over = cand;  // candidates at or above thr
-    auto count = [&](uint32_t trial) {
-      int c = 0;
+  if (want < cand && want > 0) {  // want == cand keeps all: threshold 0
+    auto each = [&](auto&& fn) {  // every key of this thread; absent ones are 0
       if (one) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) c += key[e] >= trial;
-      } else {
-        for (int j = tid; j < cand; j += kEvictThreads) c += evict_key(__ldg(sc + j)) >= trial;
-      }
-      return evict_block_sum(c, red, turn);
-    };
-    auto step = [&](int c, uint32_t trial) {  // exactly `want` reach trial: keep keys > trial - 1
-      if (c == want) {
-        thr = trial - 1;
-        exact = true;
-      } else if (c > want) {
-        thr = trial;
-        over = c;
-      }
-    };
-    for (; bit >= 32 - kEvictWideBits && !exact; --bit)
-      step(count(thr | (1u << bit)), thr | (1u << bit));
-    // keys that share the bits so far: those in [thr, thr + 2^(bit + 1))
-    const uint32_t span = 1u << (bit + 1);
-    if (!exact) {
-      if (tid == 0) list_n = 0;
-      __syncthreads();
-      auto put = [&](uint32_t k) {
-        const bool in = k - thr < span && k != 0u;
-        const unsigned mask = __ballot_sync(0xffffffffu, in);
-        int at = 0;
-        if (lane == 0 && mask) at = atomicAdd(&list_n, __popc(mask));  // order does not matter
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
-        if (in && at < kEvictList) list[at] = k;
-      };
-      if (one) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) put(key[e]);
+        for (int e = 0; e < E; ++e) fn(key[e]);
       } else {
         for (int j = tid; j - tid < cand; j += kEvictThreads)
-          put(j < cand ? evict_key(__ldg(sc + j)) : 0u);
+          fn(j < cand ? evict_key(__ldg(sc + j)) : 0u);
+      }
+    };
+    // the keys' range, and its steps
+    for (int i = tid; i < kEvictBins; i += kEvictThreads) bins[i] = 0;
+    if (tid == 0) list_n = 0;
+    uint32_t lo = 0xffffffffu, hi = 0u;
+    each([&](uint32_t k) {
+      if (k) lo = min(lo, k);
+      hi = max(hi, k);
+    });
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) {
+      list[warp] = lo;
+      list[kEvictWarps + warp] = hi;
+    }
+    __syncthreads();
+    lo = __reduce_min_sync(0xffffffffu, list[lane & (kEvictWarps - 1)]);
+    hi = __reduce_max_sync(0xffffffffu, list[kEvictWarps + (lane & (kEvictWarps - 1))]);
+    const int width = 32 - __clz((int)(hi - lo));  // bits of the range
+    const int shift = width > 11 ? width - 11 : 0;
+    each([&](uint32_t k) {
+      if (k) atomicAdd(&bins[(k - lo) >> shift], 1);  // whole numbers: any order
+    });
+    __syncthreads();
+    // the step that holds the threshold: thread t sums 4 steps, highest first
+    constexpr int PER = kEvictBins / kEvictThreads;
+    int v[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      v[i] = bins[kEvictBins - 1 - (tid * PER + i)];
+      sum += v[i];
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    int* r16 = red + turn * kEvictWarps;
+    turn ^= 1;
+    if (lane == 31) r16[warp] = inc;
+    __syncthreads();
+    int run = inc - sum;
+#pragma unroll
+    for (int w = 0; w < kEvictWarps; ++w)
+      if (w < warp) run += r16[w];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (run < want && run + v[i] >= want) {
+        s_bin = kEvictBins - 1 - (tid * PER + i);
+        s_higher = run;
+      }
+      run += v[i];
+    }
+    __syncthreads();
+    const int bin = s_bin, higher = s_higher, need = want - higher;
+    const uint32_t base = lo + ((uint32_t)bin << shift), steps = (1u << shift) - 1u;
+    // that step's keys
+    each([&](uint32_t k) {
+      const bool in = k >= base && k - base <= steps;
+      const unsigned mask = __ballot_sync(0xffffffffu, in);
+      int at = 0;
+      if (lane == 0 && mask) at = atomicAdd(&list_n, __popc(mask));  // order does not matter
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
+      if (in && at < kEvictList) list[at] = k;
+    });
+    __syncthreads();
+    const int ln = list_n;
+    if (ln <= kEvictRank) {
+      if (tid < ln) {
+        const uint32_t k = list[tid];
+        int above = 0, same = 0;
+        for (int x = 0; x < ln; ++x) {
+          above += list[x] > k;
+          same += list[x] == k;
+        }
+        if (above < need && above + same >= need) s_thr = k;  // every such thread: one value
       }
       __syncthreads();
-      const int ln = list_n, higher = over - ln;  // candidates above the list's range
-      const bool listed = ln <= kEvictList;
-      for (; bit >= 0 && !exact; --bit) {
-        const uint32_t trial = thr | (1u << bit);
-        if (listed) {
-          int c = 0;
+      thr = s_thr;
+    } else {
+      thr = base;
+      for (int bit = shift - 1; bit >= 0; --bit) {
+        const uint32_t trial = base + ((thr - base) | (1u << bit));
+        int c = 0;
+        if (ln <= kEvictList) {
           for (int j = tid; j < ln; j += kEvictThreads) c += list[j] >= trial;
-          step(evict_block_sum(c, red, turn) + higher, trial);
+          c = evict_block_sum(c, red, turn) + higher;
         } else {
-          step(count(trial), trial);
+          each([&](uint32_t k) { c += k >= trial; });
+          c = evict_block_sum(c, red, turn);
         }
+        if (c >= want) thr = trial;
       }
     }
+  } else if (want == 0) {
+    thr = 0xffffffffu;  // none of the candidates
   }
   // ties at the threshold that stay: the first `ties` of them
   int above = 0;

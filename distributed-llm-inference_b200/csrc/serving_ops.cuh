@@ -56,22 +56,24 @@ constexpr int64_t kTcRows = 33;
 
 // Ranges per item of the tcgen05 kernel (items: query tile pairs of all kv heads, with
 // `tiles` key tiles each) when the mma.sync kernel runs beside it on the SMs that
-// are left: those with the earlier end by the measured rates (a key tile 1.9 us
-// after 10 us of start and end; own contexts 0.74 us of an SM's time per 64 keys of
-// head_dim 128, its share of HBM, 0.5 at 64, after 8 us), or 0 where one after the
-// other on all SMs ends no later. Own lengths are on the device: half the bound is
-// taken. (B200, one token for 64 sequences over a prefix of 4096: 57 us in turn, 37
-// with 32 SMs for the prefix, 49 with 24, 42 with 60; 256 x 4 tokens over 8192 with
-// own contexts to 2048: 356 us in turn, 390 with half of the SMs.)
-int tc_splits(int sms, int64_t items, int64_t tiles, double own_units, int64_t D) {
-  const double own = own_units * (D == 128 ? 0.74 : 0.5);
+// are left: those with the earlier end by the measured rates, or 0 where one after
+// the other on all SMs ends no later. A key tile takes 2.4 us (head_dim 64: 1.9) after
+// 10 us of start and end; 64 keys of own contexts 0.74 us of an SM's time at 16 rows
+// or less, 1.2 at 32 (head_dim 64: 0.62), after 8 us. Own lengths are on the device:
+// half the bound is taken. (B200: one token for 64 sequences over a prefix of 4096,
+// 8 items: 53 us in turn, 42, 37, 37 and 39 with 3, 4, 5 and 6 ranges; 24 sequences
+// of 6 tokens over 2501, 24 items: 38 in turn, 40, 36, 40 with 2, 3, 4; 256 x 4 tokens
+// over 8192 with own contexts to 2048: 356 in turn, 390 with half of the SMs.)
+int tc_splits(int sms, int64_t items, int64_t tiles, double own_units, int64_t own_rows, int64_t D) {
+  const double tile = D == 128 ? 2.4 : 1.9;
+  const double own = own_units * (D == 64 ? 0.62 : own_rows <= 16 ? 0.74 : 1.2);
   const int64_t all = sms / items < 1 ? 1 : sms / items;
   const double tc_all = items * all <= sms ? (double)((tiles + all - 1) / all)
                                            : (double)(items * tiles) / sms;
-  double best = 10 + 1.9 * tc_all + 12 + own / sms;
+  double best = 10 + tile * tc_all + 12 + own / sms;
   int splits = 0;
   for (int64_t k = 1; k <= tiles && items * k < sms; ++k) {
-    const double a = 10 + 1.9 * ((tiles + k - 1) / k), b = 8 + own / (sms - items * k);
+    const double a = 10 + tile * ((tiles + k - 1) / k), b = 8 + own / (sms - items * k);
     if ((a > b ? a : b) < best) {
       best = a > b ? a : b;
       splits = (int)k;
@@ -112,7 +114,7 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
     if (pl.own_kernel == kSpanMma) {
       const int64_t r = 8 * span_nt(TG);
       pl.splits = tc_splits(sms, items, tiles,
-                            (double)(B * KVH * ((TG + r - 1) / r)) * (max_length / 128.0 + 0.3), D);
+                            (double)(B * KVH * ((TG + r - 1) / r)) * (max_length / 128.0 + 0.3), r, D);
       beside_sms = (int)items * pl.splits;
     }
     if (!pl.splits && items <= sms / 2)  // on all SMs: whole ranges where items are few
@@ -451,7 +453,7 @@ int pdb_shared_prefix_attention_impl(
   }
   if (e == cudaSuccess && scores && scores_width > 0)
     e = launch_pdl(pdb::prefix_scores_kernel,
-                   dim3((unsigned)((scores_width + 255) / 256), (unsigned)(p.B * p.KVH)),
+                   dim3((unsigned)((scores_width + 1023) / 1024), (unsigned)(p.B * p.KVH)),
                    dim3(256), 0, st, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "shared prefix attention launch");
