@@ -18,6 +18,9 @@ import torch
 from . import _lib
 from .ops import _DTYPES, _DeviceGuard, _stream_ptr, workspace
 
+_INT32, _INT64, _FP32 = torch.int32, torch.int64, torch.float32
+_current_device = torch.cuda.current_device
+
 
 def _refuse(message: str):
     raise RuntimeError(message)
@@ -32,6 +35,17 @@ def _check_same_device(device: int, *tensors) -> None:
                 _refuse("all tensors must be on the same GPU")
             if not t.is_contiguous():
                 _refuse("all tensors must be contiguous")
+
+
+def _run_on(device: int, launch, what: str) -> None:
+    """Runs `launch` with `device` current; raises on a failed call."""
+    if _current_device() == device:
+        rc = launch()
+    else:
+        with _DeviceGuard(torch.device("cuda", device)):
+            rc = launch()
+    if rc:
+        _lib.check(rc, what)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -90,13 +104,13 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         _refuse("use FP32 or FP16")
     if k.dtype != dtype or v.dtype != dtype:
         _refuse("dtype mismatch")
-    if not (tables.dtype == lengths.dtype == prefix_table.dtype == torch.int32):
+    if not (tables.dtype == lengths.dtype == prefix_table.dtype == _INT32):
         _refuse("metadata must be int32")
     if tables.dim() != 2 or tables.shape[0] != B or prefix_table.dim() != 1:
         _refuse("invalid block tables")
     if lengths.shape != (B,):
         _refuse("invalid lengths")
-    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (B,)):
+    if counts is not None and (counts.dtype != _INT32 or counts.shape != (B,)):
         _refuse("invalid token counts")
     prefix_length, max_length = int(prefix_length), int(max_length)
     pages, table_width = prefix_table.shape[0], tables.shape[1]
@@ -106,14 +120,14 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         _refuse("invalid context bound")
     width, scores_ptr, scores_out_ptr = 0, None, None
     if scores is not None:
-        if scores.dtype != torch.float32 or scores.dim() != 3 or scores.shape[:2] != (B, KVH):
+        if scores.dtype != _FP32 or scores.dim() != 3 or scores.shape[:2] != (B, KVH):
             _refuse("scores must be fp32 [batch, kv_heads, tokens]")
         width = scores.shape[2]
         if width < max_length:
             _refuse("scores must hold max_length tokens")
         if scores_out is None:
             scores_out = scores
-        elif scores_out.shape != scores.shape or scores_out.dtype != torch.float32:
+        elif scores_out.shape != scores.shape or scores_out.dtype != _FP32:
             _refuse("invalid scores output")
         if width:
             scores_ptr, scores_out_ptr = scores.data_ptr(), scores_out.data_ptr()
@@ -124,18 +138,21 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     elif not (out.shape == q_shape and out.dtype == dtype and out.is_contiguous()
               and out.get_device() == device):
         _refuse("invalid output tensor")
-    with _DeviceGuard(q.device):
-        stream = _stream_ptr(q.device)
+
+    def launch():
+        where = q.device
+        stream = _stream_ptr(where)
         need = _prefix_workspace(device, B, T, H, KVH, D, prefix_length, max_length, dt,
                                  width > 0)
-        ws = workspace(q.device, stream, need, "shared_prefix")
-        rc = _lib.load().pdb_shared_prefix_attention_impl(
+        ws = workspace(where, stream, need, "shared_prefix")
+        return _lib.load().pdb_shared_prefix_attention_impl(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), prefix_table.data_ptr(), pages,
             prefix_length, tables.data_ptr(), lengths.data_ptr(),
             counts.data_ptr() if counts is not None else None, scores_ptr, scores_out_ptr, width,
             out.data_ptr(), B, T, H, D, N, bs, KVH, table_width, max_length, dt,
             ws.data_ptr() if ws is not None else None, need, stream, impl)
-    _lib.check(rc, "shared_prefix_attention")
+
+    _run_on(device, launch, "shared_prefix_attention")
     return out if scores is None else (out, scores_out)
 
 
@@ -177,25 +194,27 @@ def verify_drafts(draft_tokens: torch.Tensor, target_probs: torch.Tensor,
             _refuse("invalid probabilities shape")
         if draft_probs.dtype != dtype:
             _refuse("dtype mismatch")
-    if draft_tokens.dtype != torch.int64:
+    if draft_tokens.dtype != _INT64:
         _refuse("draft tokens must be int64")
-    if not (accept_uniforms.dtype == sample_uniforms.dtype == torch.float32
+    if not (accept_uniforms.dtype == sample_uniforms.dtype == _FP32
             and accept_uniforms.shape == (B, T) and sample_uniforms.shape == (B,)):
         _refuse("invalid random numbers")
-    if draft_lengths is not None and (draft_lengths.dtype != torch.int32
+    if draft_lengths is not None and (draft_lengths.dtype != _INT32
                                       or draft_lengths.shape != (B,)):
         _refuse("invalid draft lengths")
     tokens = draft_tokens.new_empty((B, T + 1))
     counts = (torch.empty_like(draft_lengths) if draft_lengths is not None
-              else draft_tokens.new_empty((B,), dtype=torch.int32))
-    with _DeviceGuard(target_probs.device):
-        rc = _lib.load().pdb_verify_drafts(
+              else draft_tokens.new_empty((B,), dtype=_INT32))
+
+    def launch():
+        return _lib.load().pdb_verify_drafts(
             draft_tokens.data_ptr(), target_probs.data_ptr(),
             draft_probs.data_ptr() if draft_probs is not None else None,
             accept_uniforms.data_ptr(), sample_uniforms.data_ptr(),
             draft_lengths.data_ptr() if draft_lengths is not None else None, tokens.data_ptr(),
             counts.data_ptr(), B, T, V, dt, _stream_ptr(target_probs.device))
-    _lib.check(rc, "verify_drafts")
+
+    _run_on(device, launch, "verify_drafts")
     return tokens, counts
 
 
@@ -230,10 +249,10 @@ def evict_tokens(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor, tables:
         _refuse("invalid lengths")
     B = lengths.shape[0]
     s_shape = scores.shape
-    if not (scores.dtype == torch.float32 and len(s_shape) == 3 and s_shape[0] == B
+    if not (scores.dtype == _FP32 and len(s_shape) == 3 and s_shape[0] == B
             and s_shape[1] == KVH and s_shape[2] > 0):
         _refuse("scores must be fp32 [batch, kv_heads, tokens]")
-    if not (tables.dtype == lengths.dtype == new_tables.dtype == torch.int32):
+    if not (tables.dtype == lengths.dtype == new_tables.dtype == _INT32):
         _refuse("metadata must be int32")
     t_shape, n_shape = tables.shape, new_tables.shape
     if not (len(t_shape) == 2 and t_shape[0] == B and t_shape[1] > 0
@@ -249,11 +268,13 @@ def evict_tokens(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor, tables:
     kept = lengths.new_empty((B, KVH, budget))
     new_lengths = torch.empty_like(lengths)
     new_scores = torch.empty_like(scores)
-    with _DeviceGuard(k.device):
-        rc = _lib.load().pdb_evict_tokens(
+
+    def launch():
+        return _lib.load().pdb_evict_tokens(
             k.data_ptr(), v.data_ptr(), scores.data_ptr(), S, tables.data_ptr(),
             lengths.data_ptr(), new_tables.data_ptr(), kept.data_ptr(), new_lengths.data_ptr(),
             new_scores.data_ptr(), B, D, N, bs, KVH, t_shape[1], n_shape[1], budget, recent, dt,
             _stream_ptr(k.device))
-    _lib.check(rc, "evict_tokens")
+
+    _run_on(device, launch, "evict_tokens")
     return kept, new_lengths, new_scores
