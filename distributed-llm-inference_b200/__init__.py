@@ -20,6 +20,8 @@ Public ops (drop-in for the reference's decode path):
       keeps a cache under a budget by accumulated weight
   DevicePagedKV              TensorPagedKV (worker/llama.py:13-55) + device-resident
                              decode tables/lengths
+  PrefixBatch                speculative decoding of requests that share a prefix on a
+                             PagedLlama: the three operators above, step by step
   PagedLlama                 worker/llama.py:89-177 on these ops (CUDA-graph decode ticks)
   cuda_paged_attention(...)  the reference loader's name (worker/llama.py:77-86)
   install(llama_module)      points a worker.llama module at these ops
@@ -36,13 +38,14 @@ from ._lib import PREFIX_AUTO, PREFIX_MMA, PREFIX_SIMT, PREFIX_TCGEN05  # noqa: 
 from .serving_ops import evict_tokens, shared_prefix_attention, verify_drafts  # noqa: F401
 from .paged_kv import DevicePagedKV  # noqa: F401
 from .llama_runner import PagedLlama  # noqa: F401
+from .speculative import PrefixBatch  # noqa: F401
 from .integration import cuda_paged_attention, install, uninstall  # noqa: F401
 
 __all__ = [
     "shared_prefix_attention", "verify_drafts", "evict_tokens",
     "paged_attention", "decode_attention", "decode_attention_supported", "prefill_attention",
     "rope_kv_write", "rope_kv_write_decode",
-    "DevicePagedKV", "PagedLlama",
+    "DevicePagedKV", "PagedLlama", "PrefixBatch",
     "cuda_paged_attention", "install", "uninstall",
     "read_device_errors", "fast_grid_size", "load_library",
     "IMPL_AUTO", "IMPL_FAST", "IMPL_GENERIC", "IMPL_SIMT", "IMPL_MMA", "IMPL_TMA_STATIC",

@@ -1,0 +1,150 @@
+"""Speculative decoding of requests that share a prefix, on a bounded cache.
+
+``PrefixBatch`` drives a ``PagedLlama`` through the serving operators: a prefix
+that every request shares (an instruction, few-shot examples) is prefilled
+once; each step scores every request's drafted tokens in one pass over the
+layers (``shared_prefix_attention``: the prefix's K and V are read once for the
+batch), accepts drafts against the model's probabilities (``verify_drafts``)
+and, when a request's own cache passes its budget, keeps its most attended
+tokens (``evict_tokens``, on the weights the attention accumulated). The
+reference decodes one token per request and step over whole contexts.
+
+Cached keys carry RoPE at the position where their token was seen, so a cache
+that lost tokens keeps the others' positions; a request's next position is
+counted apart from its cache length.
+"""
+from __future__ import annotations
+
+import torch
+
+from .ops import rope_kv_write
+from .serving_ops import evict_tokens, shared_prefix_attention, verify_drafts
+
+_PREFIX = "shared prefix"
+
+
+class PrefixBatch:
+    """Requests ``ids`` that continue ``prefix`` (token ids), up to ``max_own``
+    cached own tokens each. With ``budget`` a request's own cache is cut to
+    that many tokens per layer and kv head whenever a step left it longer; the
+    last ``recent`` stay in any case."""
+
+    def __init__(self, runner, prefix, ids, max_own: int, budget: int | None = None,
+                 recent: int = 32):
+        if budget is not None and not 0 <= recent <= budget <= max_own:
+            raise ValueError("recent <= budget <= max_own is needed")
+        self.runner, self.ids, self.max_own = runner, list(ids), max_own
+        self.budget, self.recent, self.prefix_length = budget, recent, len(prefix)
+        cache = runner.cache
+        if prefix:
+            if not cache.reserve(_PREFIX, len(prefix)):
+                raise RuntimeError("the cache has no pages for the prefix")
+            runner.prefill([_PREFIX], [list(prefix)])
+        self.prefix_table = torch.tensor(cache.tables.get(_PREFIX, []), dtype=torch.int32,
+                                         device=runner.device)
+        for rid in self.ids:
+            if not cache.reserve(rid, max_own):
+                raise RuntimeError("the cache has no pages for the requests")
+        self.seen = {rid: 0 for rid in self.ids}  # own tokens so far, evicted ones included
+        layers = len(runner.model.model.layers)
+        self.scores = torch.zeros((layers, len(self.ids), runner.kv_heads, max_own),
+                                  device=runner.device) if budget is not None else None
+
+    def close(self) -> None:
+        for rid in [*self.ids, _PREFIX]:
+            self.runner.cache.release(rid)
+
+    @torch.inference_mode()
+    def score(self, token_lists) -> torch.Tensor:
+        """Appends each request's tokens (one or more, ragged) to its cache and
+        returns the logits that follow them, float32 [B, T, vocab] (rows past a
+        request's own count are meaningless)."""
+        runner, cache = self.runner, self.runner.cache
+        counts = [len(tokens) for tokens in token_lists]
+        B, T = len(self.ids), max(counts)
+        before = [cache.lengths[rid] for rid in self.ids]
+        if any(not n for n in counts) or any(b + n > self.max_own for b, n in zip(before, counts)):
+            raise ValueError("each request takes one token at least, and max_own cached in all")
+        rows = torch.tensor([list(t) + [0] * (T - len(t)) for t in token_lists])
+        first = torch.tensor([self.prefix_length + self.seen[rid] for rid in self.ids])
+        positions = (first[:, None] + torch.arange(T)).to(runner.device)
+        valid = (torch.arange(T) < torch.tensor(counts)[:, None]).to(runner.device)
+        physical, offsets = cache.slots(self.ids, [range(b, b + n) for b, n in zip(before, counts)])
+        for rid, b, n in zip(self.ids, before, counts):
+            cache.lengths[rid] = b + n
+            self.seen[rid] += n
+        tables, lengths, longest = cache.metadata(self.ids)
+        real = torch.tensor(counts, dtype=torch.int32, device=runner.device)
+        x = runner.model.model.embed_tokens(rows.to(runner.device))
+        for index, layer in enumerate(runner.model.model.layers):
+            attn = layer.self_attn
+            h = layer.input_layernorm(x)
+            q = attn.q_proj(h).view(B, T, runner.heads, runner.head_dim)
+            k = attn.k_proj(h).view(B, T, runner.kv_heads, runner.head_dim)
+            v = attn.v_proj(h).view(B, T, runner.kv_heads, runner.head_dim)
+            keys, values = cache.keys[index], cache.values[index]
+            q, _ = rope_kv_write(q, k, v.contiguous(), keys, values, physical, offsets, positions,
+                                 runner.inv_freq, valid=valid, inplace=True)
+            context = shared_prefix_attention(
+                q, keys, values, self.prefix_table, self.prefix_length, tables, lengths, longest,
+                counts=real, scores=self.scores[index] if self.scores is not None else None)
+            if self.scores is not None:
+                context = context[0]
+            x = x + attn.o_proj(context.reshape(B, T, -1))
+            x = x + layer.mlp(layer.post_attention_layernorm(x))
+        return runner.model.lm_head(runner.model.model.norm(x)).float()
+
+    @torch.inference_mode()
+    def step(self, last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs=None,
+             temperature: float = 1.0):
+        """One speculative step. ``last_tokens``: each request's newest token,
+        not cached yet; ``drafts``: up to T guessed tokens after it;
+        ``accept_uniforms`` fp32 [B, T], ``sample_uniforms`` fp32 [B];
+        ``draft_probs`` fp32 [B, T, vocab], or None for drafts that were not
+        sampled. Returns the new tokens of each request (1 to T + 1 of them):
+        distributed as the model's own, however good the drafts are."""
+        cache, device = self.runner.cache, self.runner.device
+        T = accept_uniforms.shape[1]
+        before = [cache.lengths[rid] for rid in self.ids]
+        seen = dict(self.seen)
+        logits = self.score([[a, *d] for a, d in zip(last_tokens, drafts)])
+        probs = torch.softmax(logits / temperature, -1)
+        if probs.shape[1] < T + 1:
+            probs = torch.nn.functional.pad(probs, (0, 0, 0, T + 1 - probs.shape[1]))
+        tokens, counts = verify_drafts(
+            torch.tensor([list(d) + [0] * (T - len(d)) for d in drafts], device=device),
+            probs.contiguous(), accept_uniforms, sample_uniforms, draft_probs=draft_probs,
+            draft_lengths=torch.tensor([len(d) for d in drafts], dtype=torch.int32, device=device))
+        new = [row[:n] for row, n in zip(tokens.tolist(), counts.tolist())]
+        for b, (rid, got) in enumerate(zip(self.ids, new)):
+            # the last token and the accepted drafts stay cached; cells past them are free
+            cache.lengths[rid] = before[b] + len(got)
+            self.seen[rid] = seen[rid] + len(got)
+            if self.scores is not None:
+                self.scores[:, b, :, cache.lengths[rid]:] = 0.0
+        if self.budget is not None:
+            self.evict([rid for rid in self.ids if cache.lengths[rid] > self.budget])
+        return new
+
+    @torch.inference_mode()
+    def evict(self, ids) -> None:
+        """Cuts the own caches of ``ids`` to the budget, into fresh pages."""
+        cache = self.runner.cache
+        ids = [rid for rid in ids if cache.reserve((rid, "kept"), self.max_own)]
+        if not ids:  # nothing to cut, or no free pages: the caches stay as they are
+            return
+        rows = torch.tensor([self.ids.index(rid) for rid in ids], device=self.scores.device)
+        tables, lengths, _ = cache.metadata(ids)
+        new_tables = torch.tensor([cache.tables[(rid, "kept")] for rid in ids], dtype=torch.int32,
+                                  device=tables.device)
+        for index in range(self.scores.shape[0]):
+            _, _, kept = evict_tokens(cache.keys[index], cache.values[index],
+                                      self.scores[index][rows], tables, lengths, new_tables,
+                                      self.budget, self.recent)
+            self.scores[index][rows] = kept
+        for rid in ids:
+            length = min(cache.lengths[rid], self.budget)
+            pages = cache.tables[(rid, "kept")]
+            cache.tables[(rid, "kept")] = cache.tables[rid]
+            cache.release((rid, "kept"))
+            cache.tables[rid], cache.lengths[rid] = pages, length
