@@ -334,3 +334,83 @@ def test_prefill_ops_checks_without_device(pkg):
     t = torch.zeros(1, 1, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="CUDA"):
         pkg.prefill_attention(q, kp, kp, t, t[:, 0].contiguous())
+
+
+# ---- shared-prefix attention, verification, eviction ----------------------------
+def prefix_attn(lib, **kw):
+    a = dict(pages=3, P=40, B=2, T=3, H=4, D=64, N=12, bs=16, KVH=2, W=3, longest=35, dtype=1,
+             scores=None, scores_out=None, width=0, impl=0)
+    a.update(kw)
+    return lib.pdb_shared_prefix_attention_impl(
+        None, None, None, None, a["pages"], a["P"], None, None, None, a["scores"], a["scores_out"],
+        a["width"], None, a["B"], a["T"], a["H"], a["D"], a["N"], a["bs"], a["KVH"], a["W"],
+        a["longest"], a["dtype"], None, 0, None, a["impl"])
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(B=0), "invalid query shape"),
+    (dict(T=0), "invalid query shape"),
+    (dict(D=257), "invalid query shape"),
+    (dict(bs=0), "invalid cache shape"),
+    (dict(KVH=3), "query heads must be a multiple of KV heads"),
+    (dict(dtype=2), "use FP32 or FP16"),
+    (dict(W=-1), "invalid block tables"),
+    (dict(P=49), "invalid prefix length"),
+    (dict(P=-1), "invalid prefix length"),
+    (dict(longest=49), "invalid context bound"),
+    (dict(longest=-1), "invalid context bound"),
+    (dict(B=70000), "shape too large"),
+    (dict(N=1 << 60), "shape too large"),
+    (dict(scores=64), "give both scores and their output"),
+    (dict(scores=64, scores_out=64, width=34), "scores must hold max_length tokens"),
+    (dict(impl=4), "unknown kernel selection"),
+    (dict(), "null tensor pointer"),
+])
+def test_shared_prefix_attention_argument_checks(lib, kw, msg):
+    assert prefix_attn(lib, **kw) == 1
+    assert _lib.last_error() == msg
+
+
+def test_shared_prefix_attention_workspace_of_bad_shapes_is_none(lib):
+    size = lib.pdb_shared_prefix_attention_workspace_size
+    assert size(0, 1, 4, 2, 64, 10, 10, 1, 0) == 0
+    assert size(1, 1, 4, 3, 64, 10, 10, 1, 0) == 0
+    assert size(1, 1, 4, 2, 64, -1, 10, 1, 0) == 0
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(B=0), "invalid probabilities shape"),
+    (dict(T=0), "invalid probabilities shape"),
+    (dict(V=0), "invalid probabilities shape"),
+    (dict(dtype=5), "use FP32 or FP16"),
+    (dict(V=(1 << 22) + 1), "shape too large"),
+    (dict(), "null tensor pointer"),
+])
+def test_verify_drafts_argument_checks(lib, kw, msg):
+    a = dict(B=2, T=3, V=100, dtype=0)
+    a.update(kw)
+    assert lib.pdb_verify_drafts(None, None, None, None, None, None, None, None, a["B"], a["T"],
+                                 a["V"], a["dtype"], None) == 1
+    assert _lib.last_error() == msg
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(B=0), "invalid cache shape"),
+    (dict(D=0), "invalid cache shape"),
+    (dict(dtype=3), "use FP32 or FP16"),
+    (dict(S=0), "invalid scores"),
+    (dict(W=0), "invalid block tables"),
+    (dict(B=70000), "shape too large"),
+    (dict(budget=0), "invalid budget"),
+    (dict(recent=33), "recent tokens must fit the budget"),
+    (dict(recent=-1), "recent tokens must fit the budget"),
+    (dict(W2=1), "new tables must hold the budget"),
+    (dict(), "null tensor pointer"),
+])
+def test_evict_tokens_argument_checks(lib, kw, msg):
+    a = dict(S=60, B=2, D=64, N=20, bs=16, KVH=2, W=4, W2=2, budget=32, recent=8, dtype=1)
+    a.update(kw)
+    assert lib.pdb_evict_tokens(None, None, None, a["S"], None, None, None, None, None, None, a["B"],
+                                a["D"], a["N"], a["bs"], a["KVH"], a["W"], a["W2"], a["budget"],
+                                a["recent"], a["dtype"], None) == 1
+    assert _lib.last_error() == msg

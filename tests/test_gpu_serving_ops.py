@@ -194,6 +194,86 @@ def test_workspace_contents_do_not_matter(pkg, cuda, name, impl):
     assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_pools_and_queries_at_any_address(pkg, cuda, D, dtype):
+    # tensors that start one element into their storage: no 16-byte pieces, no TMA
+    d = make(5, 3, 8, 2, D, dtype, 70, [3, 16, 17, 64, 90], scores=True)
+    aligned = call(pkg, dict(d), cuda)
+    moved = {}
+    for n in ("q", "k", "v"):
+        flat = torch.empty(d[n].numel() + 1, dtype=dtype, device=cuda)
+        moved[n] = flat[1:].view(d[n].shape)
+        moved[n].copy_(d[n])
+    for names in (("q",), ("k", "v"), ("q", "k", "v")):
+        out, sc = call(pkg, dict(d, **{n: moved[n] for n in names}), cuda)
+        tol = 3e-3 if dtype == torch.float16 else 4e-5  # two results, each within its bound
+        assert (out - aligned[0]).abs().max().item() <= tol
+        torch.testing.assert_close(sc, aligned[1], rtol=4e-5, atol=4e-6)
+    if dtype == torch.float16:
+        with pytest.raises(RuntimeError, match="shape/alignment"):
+            call(pkg, dict(d, k=moved["k"], v=moved["v"]), cuda, "mma")
+
+
+def test_cells_past_two_to_the_31_elements(pkg, cuda):
+    # pools of 4.3 GB: the last pages' cells lie past 2^31 elements
+    KVH, D, bs = 8, 128, 16
+    N = 2 ** 31 // (bs * KVH * D) + 64
+    if torch.cuda.mem_get_info()[0] < 12 * N * bs * KVH * D:
+        pytest.skip("needs 26 GB")
+    k = torch.empty(N, bs, KVH, D, dtype=torch.float16, device=cuda)
+    v = torch.empty_like(k)
+    g = torch.Generator(device=cuda).manual_seed(3)
+    for pool in (k, v):
+        pool[-64:].normal_(generator=g)
+        pool[:8].normal_(generator=g)
+    q = torch.randn(2, 2, 32, D, generator=g, device=cuda).half()
+    order = torch.randperm(60, device=cuda).to(torch.int32) + (N - 64)
+    small = torch.arange(60, dtype=torch.int32, device=cuda)
+    lengths = torch.tensor([150, 70], dtype=torch.int32, device=cuda)
+    scores = torch.rand(2, KVH, 160, generator=g, device=cuda)
+    ck, cv = k[order.long()].contiguous(), v[order.long()].contiguous()
+    for impl in ("simt", "mma", "tcgen05"):
+        far = pkg.shared_prefix_attention(q, k, v, order[:20], 310, order[20:40].view(2, 10), lengths,
+                                          150, scores=scores, scores_out=torch.empty_like(scores),
+                                          impl=impl_of(pkg, impl))
+        near = pkg.shared_prefix_attention(q, ck, cv, small[:20], 310, small[20:40].view(2, 10),
+                                           lengths, 150, scores=scores,
+                                           scores_out=torch.empty_like(scores),
+                                           impl=impl_of(pkg, impl))
+        assert torch.equal(far[0], near[0]) and torch.equal(far[1], near[1])
+    new = order[40:60].view(2, 10)
+    kept, n, _ = pkg.evict_tokens(k, v, scores, order[20:40].view(2, 10), lengths, new, 100, 5)
+    for b in range(2):
+        for h in (0, KVH - 1):
+            j = kept[b, h, :int(n[b])].long()
+            src = order[20:40].view(2, 10)[b][j // bs].long()
+            i = torch.arange(len(j), device=cuda)
+            dst = new[b][i // bs].long()
+            assert torch.equal(k[dst, i % bs, h], k[src, j % bs, h])
+            assert torch.equal(v[dst, i % bs, h], v[src, j % bs, h])
+    assert pkg.read_device_errors() == 0
+
+
+def test_calls_on_two_streams_do_not_share_scratch(pkg, cuda):
+    jobs = [make(20, 3, 8, 2, 64, torch.float16, 300, [5 + 3 * i for i in range(20)], seed=s)
+            for s in range(2)]
+    alone = [call(pkg, d, cuda) for d in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    inputs = [{n: t.to(cuda) if isinstance(t, torch.Tensor) else t for n, t in d.items()} for d in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (s, c) in enumerate(zip(streams, inputs)):
+            with torch.cuda.stream(s):
+                got[i].append(pkg.shared_prefix_attention(
+                    c["q"], c["k"], c["v"], c["prefix_table"], c["prefix"], c["tables"],
+                    c["lengths"], c["max_length"]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, alone[i]) for x in got[i])
+
+
 def test_scores_in_place_and_beside(pkg, cuda):
     d = make(3, 2, 8, 2, 64, torch.float16, 30, [4, 20, 67], scores=True)
     c = {n: t.to(cuda) if isinstance(t, torch.Tensor) else t for n, t in d.items()}
@@ -461,6 +541,36 @@ def test_evict_longer_than_one_round(pkg, cuda):
     d = cache(1, 1, 8, torch.float16, [20011], 6000, bs=64)
     d["scores"] = (d["scores"] * 4).floor()                     # many ties across rounds
     check_evict(pkg, d, cuda, 6000, 11)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
+def test_evict_rows_at_any_address(pkg, cuda, dtype):
+    # few rows (copied by the selecting CTA) and many (by a kernel of their own)
+    for lengths, budget, D in (([60, 90], 40, 64), ([700], 600, 128)):
+        d = cache(len(lengths), 2, D, dtype, lengths, budget)
+        c = {n: t.to(cuda) for n, t in d.items()}
+        want = pkg.evict_tokens(c["k"], c["v"], c["scores"], c["tables"], c["lengths"],
+                                c["new_tables"], budget, 3)
+        moved = []
+        for n in ("k", "v"):
+            flat = torch.empty(d[n].numel() + 1, dtype=dtype, device=cuda)
+            moved.append(flat[1:].view(d[n].shape))
+            moved[-1].copy_(d[n])
+        got = pkg.evict_tokens(*moved, c["scores"], c["tables"], c["lengths"], c["new_tables"],
+                               budget, 3)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        assert torch.equal(moved[0], c["k"]) and torch.equal(moved[1], c["v"])
+
+
+def test_evict_crowded_histogram_steps(pkg, cuda):
+    # one outlier stretches the keys' range, so that all others share one step of the
+    # histogram: more keys than are ranked, and more than are listed
+    for n, budget in ((1200, 700), (6000, 2500), (20000, 9000)):
+        d = cache(1, 2, 8, torch.float16, [n], budget, bs=64)
+        g = torch.Generator().manual_seed(n)
+        d["scores"] = 1.0 + torch.randint(0, 40, d["scores"].shape, generator=g) * 2.0 ** -23
+        d["scores"][0, 0, 5], d["scores"][0, 1, 7] = 3e38, -3e38
+        check_evict(pkg, d, cuda, budget, 11)
 
 
 def test_evict_bad_metadata_is_flagged_not_followed(pkg, cuda):
