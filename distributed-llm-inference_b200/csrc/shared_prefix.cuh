@@ -487,6 +487,21 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
   if (!real) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
   T* out = static_cast<T*>(p.out) + (int64_t)row * D;
+  if constexpr (VEC) {
+    if ((reinterpret_cast<uintptr_t>(p.out) & 15u) == 0) {
+      if (4 * lane < D) {
+        __align__(16) T o4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o4[i] = Elem<T>::from_f(l == 0.f ? 0.f : acc[i] * inv);
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<uint2*>(out + 4 * lane) = *reinterpret_cast<const uint2*>(o4);
+        else
+          *reinterpret_cast<uint4*>(out + 4 * lane) = *reinterpret_cast<const uint4*>(o4);
+      }
+      if (p.lse && lane == 0) p.lse[row] = l == 0.f ? INFINITY : m + log2f(l);
+      return;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int d = VEC ? 4 * lane + i : lane + 32 * i;

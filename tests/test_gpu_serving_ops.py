@@ -317,6 +317,61 @@ def test_three_dimensional_query_side_stream_and_graph(pkg, cuda):
     assert torch.equal(held, ref[:, 0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
+def test_graph_replays_of_kernels_side_by_side(pkg, cuda, dtype):
+    # a prefix kernel with the own-token kernel beside it, captured; the replays run
+    # back to back, so that a call's partials are rewritten right after they were read
+    d = make(24, 3, 8, 2, 64, dtype, 500, [3 + 11 * i for i in range(24)], scores=True)
+    c = {n: t.to(cuda) if isinstance(t, torch.Tensor) else t for n, t in d.items()}
+    beside = torch.empty_like(c["scores"])
+
+    def once(q):
+        return pkg.shared_prefix_attention(q, c["k"], c["v"], c["prefix_table"], 500, c["tables"],
+                                           c["lengths"], d["max_length"], scores=c["scores"],
+                                           scores_out=beside)[0]
+    other = torch.randn_like(c["q"])
+    want = [once(c["q"]).clone(), once(other).clone()]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        once(c["q"])
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        held = [once(q) for q in (c["q"], other) for _ in range(3)]
+    for _ in range(5):
+        for h in held:
+            h.zero_()
+        graph.replay()
+        graph.replay()
+    torch.cuda.synchronize()
+    for i, h in enumerate(held):
+        assert torch.equal(h, want[i // 3])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
+def test_a_batch_past_the_lengths_kept_in_shared_memory(pkg, cuda, dtype):
+    lengths = [(i * 37) % 41 for i in range(310)]
+    check(pkg, make(310, 1, 2, 1, 64, dtype, 33, lengths, scores=True), cuda)
+
+
+@pytest.mark.parametrize("impl", IMPLS)
+def test_accumulated_weights_without_own_tokens(pkg, cuda, impl):
+    d = make(2, 1, 4, 2, 64, torch.float16, 40, [0, 0], scores=True)
+    out, sc = call(pkg, d, cuda, impl)
+    assert torch.equal(sc.cpu(), d["scores"]) and torch.isfinite(out).all()
+
+
+def test_given_output_at_any_address(pkg, cuda):
+    d = make(3, 2, 8, 2, 64, torch.float16, 30, [4, 20, 67])
+    want = call(pkg, d, cuda)
+    flat = torch.empty(want.numel() + 1, dtype=torch.float16, device=cuda)
+    for out in (torch.empty_like(want), flat[1:].view(want.shape)):
+        assert call(pkg, d, cuda, out=out) is out and torch.equal(out, want)
+    with pytest.raises(RuntimeError, match="invalid output tensor"):
+        call(pkg, d, cuda, out=torch.empty_like(want, dtype=torch.float32))
+
+
 def test_bad_metadata_is_flagged_not_followed(pkg, cuda):
     d = make(3, 2, 4, 2, 64, torch.float16, 40, [4, 20, 30], stale=0.0)
     for name, value, bit in (("lengths", [99, -4, 30], 0x2), ("counts", [3, -1, 2], 0x2),
