@@ -439,7 +439,10 @@ int pdb_shared_prefix_attention_impl(
     e = launch_spans_simt(dev, dtype, p, false, st);
   if (e == cudaSuccess) {
     auto join = [&](auto* fn, int lanes) {
-      return launch_pdl(fn, dim3((unsigned)((p.rows * lanes + 255) / 256)), dim3(256), 0, st, p);
+      const int threads = std::min(256, (p.H * lanes + 31) / 32 * 32);
+      const dim3 grid((unsigned)(batch * tokens),
+                      (unsigned)((p.H * lanes + threads - 1) / threads));
+      return launch_pdl(fn, grid, dim3((unsigned)threads), 0, st, p);
     };
     const bool vec = head_dim % 4 == 0 && head_dim <= 128;
     if (dtype == PDB_DTYPE_FLOAT16)

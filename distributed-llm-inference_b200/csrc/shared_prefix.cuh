@@ -26,6 +26,8 @@
 // Either way a row's partials are evenly spaced: prefix_join_kernel joins them.
 #pragma once
 
+#include <type_traits>
+
 #include "attention.cuh"
 
 namespace pdb {
@@ -380,20 +382,22 @@ __device__ __forceinline__ PartRange prefix_parts(const PartSet& s, int seg, int
 // VEC: D % 4 == 0 and D <= 128, four dims per lane, LPR lanes per row (D / 4
 // rounded up to 16 or 32); else up to 8 strided dims per lane, 32 lanes. Lane i
 // takes the (m, l) of part i, so the reads of O wait for nothing but the parts'
-// places, and eight of them are in flight: with one after the other, a short call of
-// 28 parts spent 21 us here. Parts are visited in order, so the sum does not depend
+// places, and four of them are in flight: with one after the other, a short call of
+// 28 parts spent 21 us here; with eight, rows of three or four parts (the usual
+// number) execute twice the instructions (256 x 4 x 32 rows: 15 us more). Parts are visited in order, so the sum does not depend
 // on which CTA finished first.
 template <typename T, int LPR, bool VEC>
 __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) {
   grid_dependency_wait();
   launch_dependents();
   constexpr int NV = VEC ? 4 : 8;
-  int row = (int)(((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR);
+  // x: token of the batch; y and the CTA's groups of LPR lanes: query heads
   const int lane = threadIdx.x % LPR, D = p.D;
-  const bool real = row < p.rows;  // the others follow along for the shuffles
-  if (!real) row = (int)p.rows - 1;
-  const int bt = row / p.H, b = bt / p.T, t = bt - b * p.T, hq = row - bt * p.H, h = hq / p.G,
-            g = hq - h * p.G;
+  int hq = blockIdx.y * (blockDim.x / LPR) + threadIdx.x / LPR;
+  const bool real = hq < p.H;  // the others follow along for the shuffles
+  if (!real) hq = p.H - 1;
+  const int bt = blockIdx.x, b = bt / p.T, t = bt - b * p.T, h = hq / p.G, g = hq - h * p.G;
+  const int64_t row = (int64_t)bt * p.H + hq;
   int n, count;
   prefix_sequence(p, b, n, count);
   const int limit = prefix_limit(n, count, t);
@@ -457,8 +461,8 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
     int most = here;
 #pragma unroll
     for (int i = 16; i >= LPR; i >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, i));
-    constexpr int U = VEC ? 8 : 2;
-    for (int s0 = 0; s0 < most; s0 += U) {
+    auto add = [&](auto width, int s0) {  // parts s0 .. s0 + width - 1
+      constexpr int U = decltype(width)::value;
       float ws[U], f[U][NV];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -480,7 +484,9 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < NV; ++i) acc[i] = fmaf(ws[u], f[u][i], acc[i]);
-    }
+    };
+    constexpr int U = VEC ? 4 : 2;
+    for (int s0 = 0; s0 < most; s0 += U) add(std::integral_constant<int, U>{}, s0);
   }
 #pragma unroll
   for (int i = LPR / 2; i; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
