@@ -29,8 +29,8 @@ struct PrefixPlan {
   size_t prefix_ml, prefix_o, prefix_dir, own_ml, own_o, own_dir, lse_off, logits_off, total;
 };
 
-constexpr int kPrefixSimtRows = 32;
-int simt_rows(int64_t rows) { return rows <= 8 ? 8 : kPrefixSimtRows; }
+// Rows per CTA of the FP32 kernel.
+int simt_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 128 ? 32 : 64; }
 
 // Key ranges for the FP32 kernel: a multiple of 64 keys, no shorter than
 // `least`, so that `tiles` CTAs per range reach `want` CTAs where the keys allow.
@@ -177,10 +177,10 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
   return pl;
 }
 
-template <typename T, int DP, int RT>
+template <typename T, int DP, int RT, bool FULL>
 cudaError_t launch_prefix_simt(int dev, const pdb::PrefixParams& p, bool prefix, cudaStream_t st) {
   using C = pdb::PrefixSimt<DP, RT>;
-  auto* fn = &pdb::prefix_simt_kernel<T, DP, RT>;
+  auto* fn = &pdb::prefix_simt_kernel<T, DP, RT, FULL>;
   if (ctas_per_sm(dev, reinterpret_cast<const void*>(fn), C::SMEM, C::NT) <= 0)
     return cudaErrorInvalidConfiguration;
   const int64_t TG = (int64_t)p.T * p.G;
@@ -188,16 +188,23 @@ cudaError_t launch_prefix_simt(int dev, const pdb::PrefixParams& p, bool prefix,
   const int own_tiles = prefix ? 0 : (int)((TG + RT - 1) / RT);
   const int64_t gx = prefix ? (int64_t)prefix_tiles * p.prefix.slots
                             : (int64_t)p.B * own_tiles * p.own.slots;
-  const int wide = p.D % 4 == 0 && aligned16(p.k_pool) && aligned16(p.v_pool);
   return launch_pdl(fn, dim3((unsigned)gx, (unsigned)p.KVH), dim3(C::NT), C::SMEM, st, p,
-                    prefix_tiles, own_tiles, wide);
+                    prefix_tiles, own_tiles);
 }
 template <typename T, int DP>
 cudaError_t launch_prefix_simt_rows(int dev, const pdb::PrefixParams& p, bool prefix,
                                     cudaStream_t st) {
-  const int64_t rows = (prefix ? p.B : 1) * (int64_t)p.T * p.G;
-  if (simt_rows(rows) == 8) return launch_prefix_simt<T, DP, 8>(dev, p, prefix, st);
-  return launch_prefix_simt<T, DP, kPrefixSimtRows>(dev, p, prefix, st);
+  const int rt = simt_rows((prefix ? p.B : 1) * (int64_t)p.T * p.G);
+  if constexpr (sizeof(T) == 4 && DP <= 128) {
+    if (p.D == DP && aligned16(p.k_pool) && aligned16(p.v_pool)) {
+      if (rt == 8) return launch_prefix_simt<T, DP, 8, true>(dev, p, prefix, st);
+      if (rt == 32) return launch_prefix_simt<T, DP, 32, true>(dev, p, prefix, st);
+      return launch_prefix_simt<T, DP, 64, true>(dev, p, prefix, st);
+    }
+  }
+  if (rt == 8) return launch_prefix_simt<T, DP, 8, false>(dev, p, prefix, st);
+  if (rt == 32) return launch_prefix_simt<T, DP, 32, false>(dev, p, prefix, st);
+  return launch_prefix_simt<T, DP, 64, false>(dev, p, prefix, st);
 }
 // The spans of the prefix (or of own tokens) on the FP32 pipes.
 cudaError_t launch_spans_simt(int dev, int dtype, const pdb::PrefixParams& p, bool prefix,

@@ -123,10 +123,10 @@ __device__ __forceinline__ int64_t prefix_cell(const PrefixParams& p, const int3
 // (row tile, range) pairs, or own (sequence, row tile, chunk) triples; y = kv head.
 template <int DP, int RT>
 struct PrefixSimt {
-  static constexpr int NT = 128;
+  static constexpr int NT = RT == 64 ? 256 : 128;
   static constexpr int KT = DP == 64 ? 64 : DP == 128 ? 32 : 16;
   static constexpr int LD = DP + 4;          // padded row of Q and K: rows 4 banks apart
-  static constexpr int RPT = RT == 32 ? 2 : 1;
+  static constexpr int RPT = RT >= 32 ? 2 : 1;
   static constexpr int TPR = NT * RPT / RT;  // threads that share a row: 8 or 16
   static constexpr int KPT = KT / TPR;       // keys per thread of S
   static constexpr int OPT = DP / 4 / TPR;   // groups of 4 dims per thread of O
@@ -135,9 +135,11 @@ struct PrefixSimt {
       (size_t)(RT * LD + 2 * KT * LD + 2 * KT * DP + RT * LP) * sizeof(float);
 };
 
-template <typename T, int DP, int RT>
+// FULL: head_dim is DP and rows come in 16-byte pieces, so that the loops over dims
+// unroll and the next reads are under way during the multiply-adds of the last.
+template <typename T, int DP, int RT, bool FULL>
 __global__ void __launch_bounds__(PrefixSimt<DP, RT>::NT)
-prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles, int wide) {
+prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
   using C = PrefixSimt<DP, RT>;
   constexpr int NT = C::NT, KT = C::KT, LD = C::LD, RPT = C::RPT, TPR = C::TPR, KPT = C::KPT,
                 OPT = C::OPT, LP = C::LP;
@@ -146,7 +148,7 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles, int wi
   float* sk = sq + RT * LD;        // [2][KT][LD]
   float* sv = sk + 2 * KT * LD;    // [2][KT][DP]
   float* sp = sv + 2 * KT * DP;    // [RT][LP]
-  const int tid = threadIdx.x, h = blockIdx.y, D = p.D, G = p.G;
+  const int tid = threadIdx.x, h = blockIdx.y, D = FULL ? DP : p.D, G = p.G;
   const bool prefix = prefix_tiles > 0, beside = !prefix && p.beside;
   if (!beside) grid_dependency_wait();
   launch_dependents();
@@ -194,8 +196,9 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles, int wi
   auto stage = [&](int t0, int buf) {
     float* dk = sk + buf * KT * LD;
     float* dv = sv + buf * KT * DP;
-    if (sizeof(T) == 4 && wide) {
-      const int pieces = D / 4;  // 16-byte pieces of a row; those past D stay zero
+    if constexpr (FULL) {
+      constexpr int pieces = DP / 4;  // 16-byte pieces of a row
+#pragma unroll 4
       for (int i = tid; i < KT * pieces; i += NT) {
         const int j = i / pieces, c = i - j * pieces;
         const int64_t cell = t0 + j < k1 ? prefix_cell(p, table, width, t0 + j) : -1;
@@ -258,6 +261,7 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles, int wi
     for (int r = 0; r < RPT; ++r)
 #pragma unroll
       for (int i = 0; i < KPT; ++i) s[r][i] = 0.f;
+#pragma unroll 4
     for (int d = 0; d < D; d += 4) {
       float4 a[RPT];
 #pragma unroll
@@ -309,6 +313,7 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles, int wi
     // keys that this row must not see have weight 0, and a v that may be anything: in
     // the tiles that hold such keys a zero weight skips its key
     const bool mask = !prefix && t0 + KT > n - count + 1;
+#pragma unroll 2
     for (int j = 0; j < KT; j += 4) {
       float4 w4[RPT];
 #pragma unroll
