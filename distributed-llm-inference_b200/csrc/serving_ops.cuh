@@ -191,12 +191,23 @@ cudaError_t launch_prefix_simt(int dev, const pdb::PrefixParams& p, bool prefix,
   return launch_pdl(fn, dim3((unsigned)gx, (unsigned)p.KVH), dim3(C::NT), C::SMEM, st, p,
                     prefix_tiles, own_tiles);
 }
+template <int DP, int R>
+cudaError_t launch_prefix_few(int dev, const pdb::PrefixParams& p, cudaStream_t st) {
+  using C = pdb::PrefixFew<DP, R>;
+  auto* fn = &pdb::prefix_few_kernel<DP, R>;
+  if (ctas_per_sm(dev, reinterpret_cast<const void*>(fn), C::SMEM, C::NT) <= 0)
+    return cudaErrorInvalidConfiguration;
+  return launch_pdl(fn, dim3((unsigned)((int64_t)p.B * p.own.slots), (unsigned)p.KVH), dim3(C::NT),
+                    C::SMEM, st, p);
+}
 template <typename T, int DP>
 cudaError_t launch_prefix_simt_rows(int dev, const pdb::PrefixParams& p, bool prefix,
                                     cudaStream_t st) {
   const int rt = simt_rows((prefix ? p.B : 1) * (int64_t)p.T * p.G);
   if constexpr (sizeof(T) == 4 && DP <= 128) {
     if (p.D == DP && aligned16(p.k_pool) && aligned16(p.v_pool)) {
+      if (!prefix && p.T * p.G <= 4) return launch_prefix_few<DP, 4>(dev, p, st);
+      if (!prefix && p.T * p.G <= 8) return launch_prefix_few<DP, 8>(dev, p, st);
       if (rt == 8) return launch_prefix_simt<T, DP, 8, true>(dev, p, prefix, st);
       if (rt == 32) return launch_prefix_simt<T, DP, 32, true>(dev, p, prefix, st);
       return launch_prefix_simt<T, DP, 64, true>(dev, p, prefix, st);

@@ -118,15 +118,16 @@ __device__ __forceinline__ int64_t prefix_cell(const PrefixParams& p, const int3
 // cp.async; others are converted on the way). Products and sums are FP32
 // throughout: FP32 parity rules tensor cores out. A thread holds RPT rows x KPT
 // keys of S and RPT rows x OPT groups of 4 dims of O, everything read from shared
-// memory in 16-byte pieces: 10 such reads per 64 multiply-adds at 32 rows. Bound by
-// the multiply-adds at 32 rows, by HBM or latency at 8. Grid: x = the prefix's
+// memory in 16-byte pieces. Such a read takes the SM four cycles whatever it
+// reads, so the reads per multiply-add bound the kernel: 8 per 64 with 4 x 4 keys and
+// rows a thread (head_dim 128, 64 rows), 6 per 32 with 2 x 4. Grid: x = the prefix's
 // (row tile, range) pairs, or own (sequence, row tile, chunk) triples; y = kv head.
 template <int DP, int RT>
 struct PrefixSimt {
-  static constexpr int NT = RT == 64 ? 256 : 128;
+  static constexpr int NT = 128;
   static constexpr int KT = DP == 64 ? 64 : DP == 128 ? 32 : 16;
   static constexpr int LD = DP + 4;          // padded row of Q and K: rows 4 banks apart
-  static constexpr int RPT = RT >= 32 ? 2 : 1;
+  static constexpr int RPT = RT == 64 ? 4 : RT == 32 ? 2 : 1;
   static constexpr int TPR = NT * RPT / RT;  // threads that share a row: 8 or 16
   static constexpr int KPT = KT / TPR;       // keys per thread of S
   static constexpr int OPT = DP / 4 / TPR;   // groups of 4 dims per thread of O
@@ -359,6 +360,249 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
     }
   }
   if (beside) grid_dependency_wait();
+}
+
+// ---- spans of few rows on the FP32 pipes ------------------------------------------
+// FP32 with head_dim DP and at most R = 4 or 8 rows per sequence (T G), 16-byte rows:
+// decode steps, bound by HBM if shared memory is read little enough. Eight lanes
+// share a key and hold the queries' dims of their slice in registers for all R rows,
+// so a key's row costs DP / 32 reads per lane for R DP / 8 multiply-adds; a
+// butterfly that halves the rows at each step leaves lane i of the eight with row
+// i's logit. Each warp takes 8 keys of a 32-key tile with its own running maximum
+// and sum, and DP / 32 dims of all R rows of O per lane; the four warps are joined at
+// the end. Three tiles in flight by cp.async, pages looked up one key per lane.
+// (8 x 8 kv heads of 2048 to 8192 keys, head_dim 128: 171 us with the kernel above,
+// whose 3 reads per 8 multiply-adds keep shared memory busy, 85 here with the join.)
+template <int DP, int R>
+struct PrefixFew {
+  static constexpr int NT = 128, KT = 32, STAGES = 3;
+  static constexpr int SL = DP / 32;  // 16-byte pieces of a lane's slice of a row
+  static constexpr int VL = DP / 32;  // dims of O per lane
+  static constexpr int STAGE = 2 * KT * DP;
+  static constexpr size_t SMEM = (size_t)(STAGES * STAGE + 4 * 8 * R + 4 * R * 2) * sizeof(float);
+  static_assert(4 * R * DP <= STAGE, "join buffer fits a stage");
+};
+
+template <int DP, int R>
+__global__ void __launch_bounds__(PrefixFew<DP, R>::NT, 2)
+prefix_few_kernel(const PrefixParams p) {
+  using C = PrefixFew<DP, R>;
+  constexpr int KT = C::KT, STAGES = C::STAGES, SL = C::SL, VL = C::VL, NT = C::NT;
+  extern __shared__ __align__(16) float smem_f[];
+  float* sp = smem_f + STAGES * C::STAGE;  // [4 warps][8 keys][R]
+  float* sm = sp + 4 * 8 * R;              // [4][R] maxima, then [4][R] sums
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, G = p.G;
+  const int sub = lane & 7, kq = lane >> 3, row = sub % R;
+  if (!p.beside) grid_dependency_wait();
+  launch_dependents();
+  const int slot = blockIdx.x % p.own.slots, b = blockIdx.x / p.own.slots;
+  int n, count;
+  prefix_sequence(p, b, n, count);
+  const int k0 = slot * p.own.chunk, k1 = k0 + p.own.chunk < n ? k0 + p.own.chunk : n;
+  if (k0 >= k1) {
+    if (p.beside) grid_dependency_wait();
+    return;
+  }
+  const int rows = p.T * G;
+  const int32_t* table = p.tables + (int64_t)b * p.table_width;
+  const float* kp = static_cast<const float*>(p.k_pool) + (int64_t)h * DP;
+  const float* vp = static_cast<const float*>(p.v_pool) + (int64_t)h * DP;
+  auto cell_of = [&](int key) -> int64_t {
+    return key < k1 ? prefix_cell(p, table, p.table_width, key) : -1;
+  };
+  auto stage = [&](int st, int64_t cell) {  // lane j holds the cell of key j
+    float* dk = smem_f + st * C::STAGE;
+    float* dv = dk + KT * DP;
+    constexpr int PIECES = DP / 4, PER = 32 / PIECES > 0 ? 32 / PIECES : 1;  // rows per warp read
+#pragma unroll
+    for (int i = 0; i < KT / (4 * PER); ++i) {
+      const int j = (i * 4 + warp) * PER + (PIECES < 32 ? lane / PIECES : 0);
+      const int64_t at = __shfl_sync(0xffffffffu, cell, j);
+      const int c = (PIECES < 32 ? lane % PIECES : lane) * 4;
+      const int64_t e = at < 0 ? 0 : at * p.KVH * DP + c;
+      cp_async16(dk + j * DP + c, kp + e, at >= 0);  // no page, past the end: zeros
+      cp_async16(dv + j * DP + c, vp + e, at >= 0);
+    }
+  };
+  int64_t cell = cell_of(k0 + lane);
+  int next = k0;
+#pragma unroll
+  for (int st = 0; st < STAGES - 1; ++st) {
+    if (next < k1) {
+      stage(st, cell);
+      next += KT;
+      cell = cell_of(next + lane);
+    }
+    cp_async_commit();
+  }
+  // this lane's slice of the queries
+  float4 q[R][SL];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < SL; ++c) {
+      q[r][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < rows) {
+        const float* src = static_cast<const float*>(p.q) +
+                           ((int64_t)(b * p.T + r / G) * p.H + (int64_t)h * G + r % G) * DP +
+                           (c * 8 + sub) * 4;
+        q[r][c] = make_float4(src[0] * p.scale_log2, src[1] * p.scale_log2,
+                              src[2] * p.scale_log2, src[3] * p.scale_log2);
+      }
+    }
+  const int limit = row < rows ? prefix_limit(n, count, row / G) : -1;
+  float* logits = p.logits && row < rows && sub < R
+                      ? p.logits + ((int64_t)b * p.KVH + h) * p.logits_width * rows + row
+                      : nullptr;
+  float m = -INFINITY, l = 0.f, acc[R][VL];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < VL; ++i) acc[r][i] = 0.f;
+  float* pw = sp + warp * 8 * R;
+
+  int st = 0;
+  for (int t0 = k0; t0 < k1; t0 += KT, st = st + 1 == STAGES ? 0 : st + 1) {
+    cp_async_wait<STAGES - 2>();
+    __syncthreads();  // this tile landed for all; the stage before it is read
+    if (next < k1) {
+      stage(st == 0 ? STAGES - 1 : st - 1, cell);
+      next += KT;
+      cell = cell_of(next + lane);
+    }
+    cp_async_commit();
+    const float* ck = smem_f + st * C::STAGE + warp * 8 * DP;
+    const float* cv = ck + KT * DP;
+    if (t0 + warp * 8 >= k1) continue;  // none of this warp's keys (the barriers are above)
+    float s[2];
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      float x[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < SL; ++c) {
+        const float4 y =
+            *reinterpret_cast<const float4*>(ck + (pass * 4 + kq) * DP + (c * 8 + sub) * 4);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          x[r] = fmaf(q[r][c].x, y.x, x[r]);
+          x[r] = fmaf(q[r][c].y, y.y, x[r]);
+          x[r] = fmaf(q[r][c].z, y.z, x[r]);
+          x[r] = fmaf(q[r][c].w, y.w, x[r]);
+        }
+      }
+      // rows halved, partners added: lane `sub` ends with row sub % R
+#pragma unroll
+      for (int half = R / 2; half; half >>= 1) {
+        const bool up = sub & half;
+#pragma unroll
+        for (int r = 0; r < half; ++r) {
+          const float give = up ? x[r] : x[r + half];
+          x[r] = (up ? x[r + half] : x[r]) + __shfl_xor_sync(0xffffffffu, give, half);
+        }
+      }
+      if constexpr (R == 4) x[0] += __shfl_xor_sync(0xffffffffu, x[0], 4);
+      const int key = t0 + warp * 8 + pass * 4 + kq;
+      const bool seen = key < limit && key < k1;
+      if (logits && seen) logits[(int64_t)key * rows] = x[0];
+      s[pass] = seen ? x[0] : -INFINITY;
+    }
+    float top = fmaxf(s[0], s[1]);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    float alpha = 1.f;
+    if (top > m) {
+      alpha = exp2f(m - top);  // m = -inf: 0
+      m = top;
+    }
+    if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float a = __shfl_sync(0xffffffffu, alpha, r);
+#pragma unroll
+        for (int i = 0; i < VL; ++i) acc[r][i] *= a;
+      }
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    const float w0 = exp2f(s[0] - ref), w1 = exp2f(s[1] - ref);
+    l = l * alpha + (w0 + w1);
+    __syncwarp();  // the weights of the tile before are read
+    if (sub < R) {
+      pw[kq * R + row] = w0;
+      pw[(4 + kq) * R + row] = w1;
+    }
+    __syncwarp();
+    // keys that a row must not see have weight 0, and a v that may be anything
+    const bool mask = t0 + KT > n - count + 1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float w[R], v[VL];
+#pragma unroll
+      for (int r = 0; r < R; r += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(pw + k * R + r);
+        w[r] = y.x; w[r + 1] = y.y; w[r + 2] = y.z; w[r + 3] = y.w;
+      }
+      if constexpr (VL == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(cv + k * DP + lane * 4);
+        v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(cv + k * DP + lane * 2);
+        v[0] = y.x; v[1] = y.y;
+      }
+      if (mask) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (w[r] != 0.f)
+#pragma unroll
+            for (int i = 0; i < VL; ++i) acc[r][i] = fmaf(w[r], v[i], acc[r][i]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < VL; ++i) acc[r][i] = fmaf(w[r], v[i], acc[r][i]);
+      }
+    }
+  }
+  // join of the four warps
+  l += __shfl_xor_sync(0xffffffffu, l, 8);
+  l += __shfl_xor_sync(0xffffffffu, l, 16);
+  if (lane < R) {
+    sm[warp * R + lane] = m;
+    sm[4 * R + warp * R + lane] = l;
+  }
+  cp_async_wait<0>();
+  __syncthreads();  // every tile is read: the first stage takes the join
+  float* jb = smem_f;  // [4][R][DP]
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float t = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) t = fmaxf(t, sm[w * R + r]);
+    const float mine = sm[warp * R + r], a = mine == -INFINITY ? 0.f : exp2f(mine - t);
+#pragma unroll
+    for (int i = 0; i < VL; ++i) jb[(warp * R + r) * DP + lane * VL + i] = acc[r][i] * a;
+  }
+  __syncthreads();
+  for (int x = tid; x < rows * DP; x += NT) {
+    const int r = x / DP, d = x - r * DP;
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) o += jb[(w * R + r) * DP + d];
+    const int64_t at = (int64_t)slot * p.rows + (int64_t)(b * p.T + r / G) * p.H +
+                       (int64_t)h * G + r % G;
+    p.own.o[at * DP + d] = o;
+    if (d == 0) {
+      float t = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) t = fmaxf(t, sm[w * R + r]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        sum += sm[4 * R + w * R + r] * (sm[w * R + r] == -INFINITY ? 0.f : exp2f(sm[w * R + r] - t));
+      p.own.ml[at] = make_float2(t, sum);
+    }
+  }
+  if (p.beside) grid_dependency_wait();
 }
 
 // ---- join of the partials -----------------------------------------------------
