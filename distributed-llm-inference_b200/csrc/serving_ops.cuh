@@ -7,6 +7,7 @@
 
 #include "shared_prefix.cuh"
 #include "shared_prefix_mma.cuh"
+#include "shared_prefix_tf32.cuh"
 #include "shared_prefix_tc.cuh"
 #include "verify.cuh"
 #include "evict.cuh"
@@ -19,7 +20,7 @@ int page_shift(int64_t bs) {
 
 // ---- shared-prefix attention -------------------------------------------------
 // The kernel of one key set: the FP32 pipes, warp-level tensor cores, tcgen05.
-enum SpanKernel { kSpanNone = 0, kSpanSimt, kSpanMma, kSpanTc };
+enum SpanKernel { kSpanNone = 0, kSpanSlots, kSpanMma, kSpanTc };
 
 struct PrefixPlan {
   int prefix_kernel, own_kernel;
@@ -29,8 +30,10 @@ struct PrefixPlan {
   size_t prefix_ml, prefix_o, prefix_dir, own_ml, own_o, own_dir, lse_off, logits_off, total;
 };
 
-// Rows per CTA of the FP32 kernel.
+// Rows per CTA of the FP32-pipe kernel, and of the TF32 kernel. Key ranges are cut for
+// the latter's.
 int simt_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 128 ? 32 : 64; }
+int slot_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 // Key ranges for the FP32 kernel: a multiple of 64 keys, no shorter than
 // `least`, so that `tiles` CTAs per range reach `want` CTAs where the keys allow.
@@ -86,8 +89,8 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
                        int64_t max_length, bool scored, bool tensor_cores, int impl) {
   PrefixPlan pl{};
   const int64_t G = H / KVH, TG = T * G, rows = B * T * H, all = B * TG;
-  pl.prefix_kernel = P <= 0 ? kSpanNone : kSpanSimt;
-  pl.own_kernel = max_length <= 0 ? kSpanNone : kSpanSimt;
+  pl.prefix_kernel = P <= 0 ? kSpanNone : kSpanSlots;
+  pl.own_kernel = max_length <= 0 ? kSpanNone : kSpanSlots;
   // unit and segment counts are 32-bit in the tensor-core kernels
   if (B * KVH * T * G * ((P + 63) / 64 + (max_length + 63) / 64 + 2) >= (int64_t(1) << 31))
     tensor_cores = false;
@@ -101,8 +104,8 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
   }
   size_t prefix_parts = 0, own_parts = 0, span_segments = 0;  // own_parts: of the mma.sync launch
   int beside_sms = 0;
-  if (pl.prefix_kernel == kSpanSimt) {
-    split_keys(P, (all + simt_rows(all) - 1) / simt_rows(all) * KVH, 4 * (int64_t)sms, 64, &pl.prefix);
+  if (pl.prefix_kernel == kSpanSlots) {
+    split_keys(P, (all + slot_rows(all) - 1) / slot_rows(all) * KVH, 4 * (int64_t)sms, 64, &pl.prefix);
     prefix_parts = (size_t)pl.prefix.slots * rows;
   } else if (pl.prefix_kernel == kSpanTc) {
     pdb::PartSet& s = pl.prefix;
@@ -122,8 +125,8 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
     s.grid = (int)(pl.splits ? items * pl.splits : std::min<int64_t>(sms, items * tiles));
     prefix_parts = (size_t)(KVH * s.segments + s.grid) * s.R;
   }
-  if (pl.own_kernel == kSpanSimt) {
-    split_keys(max_length, (TG + simt_rows(TG) - 1) / simt_rows(TG) * B * KVH, 8 * (int64_t)sms, 128,
+  if (pl.own_kernel == kSpanSlots) {
+    split_keys(max_length, (TG + slot_rows(TG) - 1) / slot_rows(TG) * B * KVH, 8 * (int64_t)sms, 128,
                &pl.own);
     own_parts = (size_t)pl.own.slots * rows;
   }
@@ -177,15 +180,29 @@ PrefixPlan prefix_plan(int sms, int64_t B, int64_t T, int64_t H, int64_t KVH, in
   return pl;
 }
 
-template <typename T, int DP, int RT, bool FULL>
+template <typename T, int DP, int RT>
 cudaError_t launch_prefix_simt(int dev, const pdb::PrefixParams& p, bool prefix, cudaStream_t st) {
   using C = pdb::PrefixSimt<DP, RT>;
-  auto* fn = &pdb::prefix_simt_kernel<T, DP, RT, FULL>;
+  auto* fn = &pdb::prefix_simt_kernel<T, DP, RT>;
   if (ctas_per_sm(dev, reinterpret_cast<const void*>(fn), C::SMEM, C::NT) <= 0)
     return cudaErrorInvalidConfiguration;
   const int64_t TG = (int64_t)p.T * p.G;
   const int prefix_tiles = prefix ? (int)((p.B * TG + RT - 1) / RT) : 0;
   const int own_tiles = prefix ? 0 : (int)((TG + RT - 1) / RT);
+  const int64_t gx = prefix ? (int64_t)prefix_tiles * p.prefix.slots
+                            : (int64_t)p.B * own_tiles * p.own.slots;
+  return launch_pdl(fn, dim3((unsigned)gx, (unsigned)p.KVH), dim3(C::NT), C::SMEM, st, p,
+                    prefix_tiles, own_tiles);
+}
+template <int D, int KW>
+cudaError_t launch_prefix_tf32(int dev, const pdb::PrefixParams& p, bool prefix, cudaStream_t st) {
+  using C = pdb::SpanTf32<D, KW>;
+  auto* fn = &pdb::prefix_tf32_kernel<C>;
+  if (ctas_per_sm(dev, reinterpret_cast<const void*>(fn), C::SMEM, C::NT) <= 0)
+    return cudaErrorInvalidConfiguration;
+  const int64_t TG = (int64_t)p.T * p.G;
+  const int prefix_tiles = prefix ? (int)((p.B * TG + C::RT - 1) / C::RT) : 0;
+  const int own_tiles = prefix ? 0 : (int)((TG + C::RT - 1) / C::RT);
   const int64_t gx = prefix ? (int64_t)prefix_tiles * p.prefix.slots
                             : (int64_t)p.B * own_tiles * p.own.slots;
   return launch_pdl(fn, dim3((unsigned)gx, (unsigned)p.KVH), dim3(C::NT), C::SMEM, st, p,
@@ -204,27 +221,31 @@ template <typename T, int DP>
 cudaError_t launch_prefix_simt_rows(int dev, const pdb::PrefixParams& p, bool prefix,
                                     cudaStream_t st) {
   const int rt = simt_rows((prefix ? p.B : 1) * (int64_t)p.T * p.G);
-  if constexpr (sizeof(T) == 4 && DP <= 128) {
-    if (p.D == DP && aligned16(p.k_pool) && aligned16(p.v_pool)) {
-      if (!prefix && p.T * p.G <= 4) return launch_prefix_few<DP, 4>(dev, p, st);
-      if (!prefix && p.T * p.G <= 8) return launch_prefix_few<DP, 8>(dev, p, st);
-      if (rt == 8) return launch_prefix_simt<T, DP, 8, true>(dev, p, prefix, st);
-      if (rt == 32) return launch_prefix_simt<T, DP, 32, true>(dev, p, prefix, st);
-      return launch_prefix_simt<T, DP, 64, true>(dev, p, prefix, st);
-    }
-  }
-  if (rt == 8) return launch_prefix_simt<T, DP, 8, false>(dev, p, prefix, st);
-  if (rt == 32) return launch_prefix_simt<T, DP, 32, false>(dev, p, prefix, st);
-  return launch_prefix_simt<T, DP, 64, false>(dev, p, prefix, st);
+  if (rt == 8) return launch_prefix_simt<T, DP, 8>(dev, p, prefix, st);
+  if (rt == 32) return launch_prefix_simt<T, DP, 32>(dev, p, prefix, st);
+  return launch_prefix_simt<T, DP, 64>(dev, p, prefix, st);
 }
-// The spans of the prefix (or of own tokens) on the FP32 pipes.
-cudaError_t launch_spans_simt(int dev, int dtype, const pdb::PrefixParams& p, bool prefix,
-                              cudaStream_t st) {
+template <int D>
+cudaError_t launch_spans_fp32(int dev, const pdb::PrefixParams& p, bool prefix, cudaStream_t st) {
+  const int64_t rows = (prefix ? p.B : 1) * (int64_t)p.T * p.G;
+  if (!prefix && rows <= 4) return launch_prefix_few<D, 4>(dev, p, st);
+  if (!prefix && rows <= 8) return launch_prefix_few<D, 8>(dev, p, st);
+  const int rt = slot_rows(rows);
+  if (rt == 16) return launch_prefix_tf32<D, 4>(dev, p, prefix, st);
+  if (rt == 32) return launch_prefix_tf32<D, 2>(dev, p, prefix, st);
+  return launch_prefix_tf32<D, 1>(dev, p, prefix, st);
+}
+// The spans of the prefix (or of own tokens) where key ranges are slots. `pieces`: FP32 with
+// rows of 16-byte pieces and the kernels made for it (head_dim 64, 128) not ruled out.
+cudaError_t launch_spans_slots(int dev, int dtype, const pdb::PrefixParams& p, bool prefix,
+                               bool pieces, cudaStream_t st) {
   if (dtype == PDB_DTYPE_FLOAT16) {
     if (p.D <= 64) return launch_prefix_simt_rows<__half, 64>(dev, p, prefix, st);
     if (p.D <= 128) return launch_prefix_simt_rows<__half, 128>(dev, p, prefix, st);
     return launch_prefix_simt_rows<__half, 256>(dev, p, prefix, st);
   }
+  if (pieces && p.D == 64) return launch_spans_fp32<64>(dev, p, prefix, st);
+  if (pieces && p.D == 128) return launch_spans_fp32<128>(dev, p, prefix, st);
   if (p.D <= 64) return launch_prefix_simt_rows<float, 64>(dev, p, prefix, st);
   if (p.D <= 128) return launch_prefix_simt_rows<float, 128>(dev, p, prefix, st);
   return launch_prefix_simt_rows<float, 256>(dev, p, prefix, st);
@@ -398,8 +419,10 @@ int pdb_shared_prefix_attention_impl(
   int dev = 0;
   int rc = current_device(&dev);
   if (rc) return rc;
-  const bool tensor_cores = prefix_tensor_cores(head_dim, num_blocks, block_size, dtype) &&
-                            aligned16(q) && aligned16(k_pool) && aligned16(v_pool);
+  const bool aligned = aligned16(q) && aligned16(k_pool) && aligned16(v_pool);
+  const bool tensor_cores =
+      prefix_tensor_cores(head_dim, num_blocks, block_size, dtype) && aligned;
+  const bool pieces = aligned && impl != PDB_PREFIX_SIMT;
   if (impl > PDB_PREFIX_SIMT && !tensor_cores)
     return fail(PDB_ERR_INVALID_ARGUMENT, "tensor-core kernels do not support this shape/alignment");
   const PrefixPlan pl = prefix_plan(sm_count(dev), batch, tokens, heads, kv_heads, head_dim,
@@ -436,7 +459,7 @@ int pdb_shared_prefix_attention_impl(
   p.table_width = (int)table_width;
   p.prefix_length = (int)prefix_length; p.max_length = (int)max_length;
   p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
-  p.beside = (pl.prefix_kernel == kSpanTc || pl.prefix_kernel == kSpanSimt) && pl.own_kernel;
+  p.beside = (pl.prefix_kernel == kSpanTc || pl.prefix_kernel == kSpanSlots) && pl.own_kernel;
   CUtensorMap kmap, vmap, kunits, vunits;  // boxes of the tcgen05 kernel, of the mma.sync kernel
   const bool tc = pl.prefix_kernel == kSpanTc;
   const bool mma = pl.prefix_kernel == kSpanMma || pl.own_kernel == kSpanMma;
@@ -449,12 +472,12 @@ int pdb_shared_prefix_attention_impl(
   if (pl.prefix_kernel == kSpanTc)
     e = head_dim == 64 ? launch_prefix_tc<64>(dev, p, pl.splits, st, kmap, vmap)
                        : launch_prefix_tc<128>(dev, p, pl.splits, st, kmap, vmap);
-  else if (pl.prefix_kernel == kSpanSimt)
-    e = launch_spans_simt(dev, dtype, p, true, st);
+  else if (pl.prefix_kernel == kSpanSlots)
+    e = launch_spans_slots(dev, dtype, p, true, pieces, st);
   if (e == cudaSuccess && mma)
     e = launch_spans_mma(dev, p, pl, st, kunits, vunits);
-  else if (e == cudaSuccess && pl.own_kernel == kSpanSimt)
-    e = launch_spans_simt(dev, dtype, p, false, st);
+  else if (e == cudaSuccess && pl.own_kernel == kSpanSlots)
+    e = launch_spans_slots(dev, dtype, p, false, pieces, st);
   if (e == cudaSuccess) {
     auto join = [&](auto* fn, int lanes) {
       const int threads = std::min(256, (p.H * lanes + 31) / 32 * 32);

@@ -15,7 +15,7 @@
 // are [b T G, (b + 1) T G). A partial is (m, l) and O of some rows over a key
 // range, in FP32: ml [..] float2, o [..][D]. The prefix's partials and those of
 // own tokens are two sets (PartSet), each written by one of these kernels:
-//   * the FP32 kernel here: fixed key ranges ("slots") of every row,
+//   * the kernels here and the TF32 kernel: fixed key ranges ("slots") of every row,
 //     part index = slot * rows + global row (b T + t) H + h;
 //   * the tensor-core kernels: work in units (64- or 128-key tiles of a segment
 //     of rows), cut into one contiguous range per CTA; CTA c's piece of segment
@@ -112,11 +112,49 @@ __device__ __forceinline__ int64_t prefix_cell(const PrefixParams& p, const int3
   return (int64_t)page * p.block_size + (tok - pi * p.block_size);
 }
 
+// The rows and keys of a CTA of the kernels with slots, by blockIdx.x: the prefix's
+// (row tile, range) pairs, or own (sequence, row tile, range) triples.
+struct SpanTile {
+  int slot, b;           // b: sequence, or -1 (the prefix)
+  int k0, k1;            // keys; none: k0 >= k1
+  int n, count;          // of the sequence
+  int r0, rend, token0;  // rows [r0, rend) as tokens from token0, heads inner
+  const int32_t* table;
+  int width;
+};
+__device__ __forceinline__ SpanTile span_tile(const PrefixParams& p, const PartSet& set,
+                                              bool prefix, int own_tiles, int rt) {
+  SpanTile t;
+  int x = blockIdx.x;
+  t.slot = x % set.slots;
+  x /= set.slots;
+  t.count = 0;
+  if (prefix) {
+    t.b = -1;
+    t.r0 = x * rt;
+    t.token0 = 0;
+    t.rend = p.B * p.T * p.G;
+    t.n = p.prefix_length;
+    t.table = p.prefix_table;
+    t.width = (p.prefix_length + p.block_size - 1) / p.block_size;
+  } else {
+    t.b = x / own_tiles;
+    prefix_sequence(p, t.b, t.n, t.count);
+    t.r0 = x % own_tiles * rt;
+    t.token0 = t.b * p.T;
+    t.rend = p.T * p.G;
+    t.table = p.tables + (int64_t)t.b * p.table_width;
+    t.width = p.table_width;
+  }
+  t.k0 = t.slot * set.chunk;
+  t.k1 = t.k0 + set.chunk < t.n ? t.k0 + set.chunk : t.n;
+  return t;
+}
+
 // ---- spans on the FP32 pipes (any type, head_dim <= DP, block size, alignment) --
 // One CTA per (row tile of RT, kv head, key range), keys in tiles of KT staged
-// in shared memory as FP32, two tiles in flight (FP32 pools with 16-byte rows:
-// cp.async; others are converted on the way). Products and sums are FP32
-// throughout: FP32 parity rules tensor cores out. A thread holds RPT rows x KPT
+// in shared memory as FP32, two tiles in flight. Products and sums are FP32
+// throughout. A thread holds RPT rows x KPT
 // keys of S and RPT rows x OPT groups of 4 dims of O, everything read from shared
 // memory in 16-byte pieces. Such a read takes the SM four cycles whatever it
 // reads, so the reads per multiply-add bound the kernel: 8 per 64 with 4 x 4 keys and
@@ -136,9 +174,7 @@ struct PrefixSimt {
       (size_t)(RT * LD + 2 * KT * LD + 2 * KT * DP + RT * LP) * sizeof(float);
 };
 
-// FULL: head_dim is DP and rows come in 16-byte pieces, so that the loops over dims
-// unroll and the next reads are under way during the multiply-adds of the last.
-template <typename T, int DP, int RT, bool FULL>
+template <typename T, int DP, int RT>
 __global__ void __launch_bounds__(PrefixSimt<DP, RT>::NT)
 prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
   using C = PrefixSimt<DP, RT>;
@@ -149,44 +185,22 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
   float* sk = sq + RT * LD;        // [2][KT][LD]
   float* sv = sk + 2 * KT * LD;    // [2][KT][DP]
   float* sp = sv + 2 * KT * DP;    // [RT][LP]
-  const int tid = threadIdx.x, h = blockIdx.y, D = FULL ? DP : p.D, G = p.G;
+  const int tid = threadIdx.x, h = blockIdx.y, D = p.D, G = p.G;
   const bool prefix = prefix_tiles > 0, beside = !prefix && p.beside;
   if (!beside) grid_dependency_wait();
   launch_dependents();
 
-  // this CTA's rows, keys and slot
-  int x = blockIdx.x, b = -1, slot, k0, k1, n = 0, count = 0, width, t0r;
-  int rend;  // rows of this tile, as tokens from token t0r, heads inner
-  const int32_t* table;
   const PartSet& set = prefix ? p.prefix : p.own;
-  slot = x % set.slots;
-  x /= set.slots;
-  int r0;
-  if (prefix) {
-    r0 = x * RT;
-    t0r = 0;
-    rend = p.B * p.T * G;
-    n = p.prefix_length;
-    table = p.prefix_table;
-    width = (p.prefix_length + p.block_size - 1) / p.block_size;
-  } else {
-    const int tile = x % own_tiles;
-    b = x / own_tiles;
-    prefix_sequence(p, b, n, count);
-    r0 = tile * RT;
-    t0r = b * p.T;
-    rend = p.T * G;
-    table = p.tables + (int64_t)b * p.table_width;
-    width = p.table_width;
-  }
-  k0 = slot * set.chunk;
-  k1 = k0 + set.chunk < n ? k0 + set.chunk : n;
+  const SpanTile t = span_tile(p, set, prefix, own_tiles, RT);
+  const int slot = t.slot, b = t.b, k0 = t.k0, k1 = t.k1, n = t.n, count = t.count,
+            width = t.width, r0 = t.r0, rend = t.rend;
+  const int32_t* table = t.table;
   if (k0 >= k1) {
     if (beside) grid_dependency_wait();
     return;
   }
   auto global_row = [&](int row) {  // of q and out
-    return (int64_t)(t0r + row / G) * p.H + (int64_t)h * G + row % G;
+    return (int64_t)(t.token0 + row / G) * p.H + (int64_t)h * G + row % G;
   };
   const T* q = static_cast<const T*>(p.q);
   const T* kp = static_cast<const T*>(p.k_pool);
@@ -197,26 +211,14 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
   auto stage = [&](int t0, int buf) {
     float* dk = sk + buf * KT * LD;
     float* dv = sv + buf * KT * DP;
-    if constexpr (FULL) {
-      constexpr int pieces = DP / 4;  // 16-byte pieces of a row
 #pragma unroll 4
-      for (int i = tid; i < KT * pieces; i += NT) {
-        const int j = i / pieces, c = i - j * pieces;
-        const int64_t cell = t0 + j < k1 ? prefix_cell(p, table, width, t0 + j) : -1;
-        const int64_t at = cell < 0 ? 0 : (cell * p.KVH + h) * D + c * 4;
-        cp_async16(dk + j * LD + c * 4, kp + at, cell >= 0);
-        cp_async16(dv + j * DP + c * 4, vp + at, cell >= 0);
-      }
-    } else {
-      for (int i = tid; i < KT * D; i += NT) {
-        const int j = i / D, d = i - j * D;
-        const int64_t cell = t0 + j < k1 ? prefix_cell(p, table, width, t0 + j) : -1;
-        const int64_t at = (cell * p.KVH + h) * D + d;
-        dk[j * LD + d] = cell < 0 ? 0.f : Elem<T>::to_f(kp[at]);
-        dv[j * DP + d] = cell < 0 ? 0.f : Elem<T>::to_f(vp[at]);
-      }
+    for (int i = tid; i < KT * D; i += NT) {
+      const int j = i / D, d = i % D;
+      const int64_t cell = t0 + j < k1 ? prefix_cell(p, table, width, t0 + j) : -1;
+      const int64_t at = (cell * p.KVH + h) * D + d;
+      dk[j * LD + d] = cell < 0 ? 0.f : Elem<T>::to_f(kp[at]);
+      dv[j * DP + d] = cell < 0 ? 0.f : Elem<T>::to_f(vp[at]);
     }
-    cp_async_commit();
   };
   if (D < DP) {  // dims past D are never staged
     for (int i = tid; i < 2 * KT * LD; i += NT) sk[i] = 0.f;
@@ -224,6 +226,7 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
     __syncthreads();
   }
   stage(k0, 0);
+#pragma unroll 8
   for (int i = tid; i < RT * DP; i += NT) {
     const int r = i / DP, d = i % DP;
     float v = 0.f;
@@ -248,12 +251,7 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
 
   int buf = 0;
   for (int t0 = k0; t0 < k1; t0 += KT, buf ^= 1) {
-    if (t0 + KT < k1) {
-      stage(t0 + KT, buf ^ 1);
-      cp_async_wait<1>();
-    } else {
-      cp_async_wait<0>();
-    }
+    if (t0 + KT < k1) stage(t0 + KT, buf ^ 1);
     __syncthreads();
     const float* ck = sk + buf * KT * LD;
     const float* cv = sv + buf * KT * DP;
@@ -363,7 +361,7 @@ prefix_simt_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
 }
 
 // ---- spans of few rows on the FP32 pipes ------------------------------------------
-// FP32 with head_dim DP and at most R = 4 or 8 rows per sequence (T G), 16-byte rows:
+// FP32 with head_dim DP and at most R = 4 or 8 rows per sequence (T G), 16-byte pieces:
 // decode steps, bound by HBM if shared memory is read little enough. Eight lanes
 // share a key and hold the queries' dims of their slice in registers for all R rows,
 // so a key's row costs DP / 32 reads per lane for R DP / 8 multiply-adds; a

@@ -179,6 +179,53 @@ def test_a_later_draft_never_reaches_an_earlier_one(pkg, cuda, dtype, impl):
         assert not torch.isfinite(got[:, 3]).any()
 
 
+OWN_ROWS = {
+    # name: (B, T, H, KVH, D, prefix, lengths, bs, counts); T G = 9, 16, 20, 32, 48, 80
+    "9 rows": (3, 3, 9, 3, 64, 33, [3, 40, 129], 16, None),
+    "16 rows": (2, 4, 8, 2, 128, 0, [4, 300], 16, [4, 2]),
+    "20 rows": (2, 5, 8, 2, 64, 20, [31, 33], 1, None),
+    "32 rows": (3, 8, 8, 2, 128, 100, [8, 95, 260], 16, [8, 8, 1]),
+    "48 rows": (2, 12, 8, 2, 128, 10, [12, 140], 12, None),
+    "80 rows": (2, 20, 8, 2, 64, 70, [19, 400], 16, [19, 20]),
+}
+
+
+@pytest.mark.parametrize("impl", ["auto", "simt"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
+@pytest.mark.parametrize("name", OWN_ROWS)
+def test_rows_of_a_sequence(pkg, cuda, name, dtype, impl):
+    B, T, H, KVH, D, prefix, lengths, bs, counts = OWN_ROWS[name]
+    check(pkg, make(B, T, H, KVH, D, dtype, prefix, lengths, bs, counts, scores=True), cuda, impl)
+
+
+@pytest.mark.parametrize("impl", ["auto", "simt"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,H,KVH,B", [(1, 4, 2, 2), (2, 8, 1, 2), (3, 8, 1, 2), (7, 16, 1, 2)])
+def test_infinities_that_every_row_sees(pkg, cuda, T, H, KVH, B, D, impl):
+    # FP32 arithmetic keeps them: V's go into their own dim only, and a key whose logit
+    # is -inf has no weight, whatever the other keys of its tile are
+    lengths = [T + 37] * B
+    d = make(B, T, H, KVH, D, torch.float32, 70, lengths)
+    d["q"][..., 1] = d["q"][..., 1].abs() + 0.5
+    for n in (5, 40):
+        at = int(d["prefix_table"][n // 16]), n % 16
+        d["v"][at][:, 3] = float("inf")
+        at = int(d["prefix_table"][n // 16]), (n + 1) % 16
+        d["k"][at][:, 1] = float("-inf")
+    for b in range(B):
+        at = int(d["tables"][b, 1]), 2
+        d["v"][at][:, 7] = float("-inf")
+        at = int(d["tables"][b, 0]), 3
+        d["k"][at][:, 1] = float("-inf")
+    out = call(pkg, d, cuda, impl).cpu()
+    ref, _ = oracle.shared_prefix_attention(d["q"], d["k"], d["v"], d["prefix_table"], d["prefix"],
+                                            d["tables"], d["lengths"], d["counts"], None)
+    assert (out[..., 3] == float("inf")).all() and (out[..., 7] == float("-inf")).all()
+    keep = [i for i in range(D) if i not in (3, 7)]
+    top = d["v"][torch.isfinite(d["v"])].abs().max().item()
+    assert (out[..., keep].double() - ref[..., keep]).abs().max().item() <= TOL[out.dtype] * top
+
+
 @pytest.mark.parametrize("name", ["nothing to see", "ragged drafts", "long drafts", "many rows"])
 @pytest.mark.parametrize("impl", IMPLS)
 def test_workspace_contents_do_not_matter(pkg, cuda, name, impl):
