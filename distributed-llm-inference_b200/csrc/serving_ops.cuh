@@ -19,7 +19,8 @@ int page_shift(int64_t bs) {
 }
 
 // ---- shared-prefix attention -------------------------------------------------
-// The kernel of one key set: the FP32 pipes, warp-level tensor cores, tcgen05.
+// The kernel of one key set: those with key ranges as slots (FP32 pipes, TF32, few rows),
+// mma.sync over FP16, tcgen05.
 enum SpanKernel { kSpanNone = 0, kSpanSlots, kSpanMma, kSpanTc };
 
 struct PrefixPlan {

@@ -73,8 +73,9 @@ typedef enum {
 
 /* Kernel selection for pdb_shared_prefix_attention_impl. */
 typedef enum {
-  PDB_PREFIX_AUTO = 0,   /* by shape                                            */
-  PDB_PREFIX_SIMT = 1,   /* FP32 arithmetic throughout, any shape               */
+  PDB_PREFIX_AUTO = 0,   /* by shape; FP32 with head_dim 64/128: TF32 in three
+                            products, with the accuracy of FP32                 */
+  PDB_PREFIX_SIMT = 1,   /* plain FP32 arithmetic throughout, any shape         */
   PDB_PREFIX_MMA = 2,    /* TMA-fed mma.sync for the prefix and own tokens: FP16,
                             head_dim 64/128, block_size % 16 == 0               */
   PDB_PREFIX_TCGEN05 = 3 /* tcgen05.mma for the prefix, mma.sync for own tokens  */
