@@ -77,23 +77,24 @@ constexpr int64_t kTcRows = 33;
 // Ranges per item of the tcgen05 kernel (items: query tile pairs of all kv heads, with
 // `tiles` key tiles each) when the mma.sync kernel runs beside it on the SMs that
 // are left: those with the earlier end by the measured rates, or 0 where one after
-// the other on all SMs ends no later. A key tile takes 2.4 us (head_dim 64: 1.9) after
-// 10 us of start and end; 64 keys of own contexts 0.74 us of an SM's time at 16 rows
-// or less, 1.2 at 32 (head_dim 64: 0.62), after 8 us. Own lengths are on the device:
+// the other on all SMs ends no later. A key tile takes 2.6 us (head_dim 64: 1.9) after
+// 8 us of start and end; 64 keys of own contexts 0.74 us of an SM's time at 16 rows
+// or less, 1.2 at 32 (head_dim 64: 0.62), after 9 us. Own lengths are on the device:
 // half the bound is taken. (B200: one token for 64 sequences over a prefix of 4096,
-// 8 items: 53 us in turn, 42, 37, 37 and 39 with 3, 4, 5 and 6 ranges; 24 sequences
-// of 6 tokens over 2501, 24 items: 38 in turn, 40, 36, 40 with 2, 3, 4; 256 x 4 tokens
-// over 8192 with own contexts to 2048: 356 in turn, 390 with half of the SMs.)
+// 8 items: 55 us in turn, 45, 39, 38 and 39 with 3, 4, 5 and 6 ranges; 24 sequences
+// of 6 tokens over 2501, 24 items: 40 in turn, 47, 42, 45 with 2, 3, 4; 128 of 5 tokens and
+// 9 heads of 64 dims over 1999: 38 in turn, 48, 35, 37 with 1, 2, 3. Over 14 shapes the
+// rule's choice costs 2% more than the best on average, 8% at most.)
 int tc_splits(int sms, int64_t items, int64_t tiles, double own_units, int64_t own_rows, int64_t D) {
-  const double tile = D == 128 ? 2.4 : 1.9;
+  const double tile = D == 128 ? 2.6 : 1.9;
   const double own = own_units * (D == 64 ? 0.62 : own_rows <= 16 ? 0.74 : 1.2);
   const int64_t all = sms / items < 1 ? 1 : sms / items;
   const double tc_all = items * all <= sms ? (double)((tiles + all - 1) / all)
                                            : (double)(items * tiles) / sms;
-  double best = 10 + tile * tc_all + 12 + own / sms;
+  double best = 8 + tile * tc_all + 10 + own / sms;
   int splits = 0;
   for (int64_t k = 1; k <= tiles && items * k < sms; ++k) {
-    const double a = 10 + tile * ((tiles + k - 1) / k), b = 8 + own / (sms - items * k);
+    const double a = 8 + tile * ((tiles + k - 1) / k), b = 9 + own / (sms - items * k);
     if ((a > b ? a : b) < best) {
       best = a > b ? a : b;
       splits = (int)k;
@@ -273,7 +274,7 @@ cudaError_t launch_spans_slots(int dev, int dtype, const pdb::PrefixParams& p, b
 template <int D, int NT, int RW>
 cudaError_t launch_span_mma(int dev, const pdb::PrefixParams& p, const pdb::SpanSet& ss, int grid,
                             cudaStream_t st, const CUtensorMap& kmap, const CUtensorMap& vmap) {
-  using C = pdb::SpanMma<D, NT, RW, (D == 128 && RW == 2) ? 2 : 3, NT == 1>;
+  using C = pdb::SpanMma<D, NT, RW, (D == 128 && RW == 2) ? 2 : 3>;
   auto* fn = &pdb::prefix_span_kernel<C>;
   if (ctas_per_sm(dev, reinterpret_cast<const void*>(fn), C::SMEM, C::THREADS) <= 0)
     return cudaErrorInvalidConfiguration;

@@ -22,10 +22,9 @@
 //     2700 at 32 rows). S^T = K Q^T (keys are the M of the product, so 8 rows
 //     cost no more than one), softmax in base 2 with the running maximum raised
 //     only when a logit passes it by 2^8 (exact after the division; weights stay
-//     below 2^8 in FP16), O^T += V^T P^T. P is rounded to FP16, an error of at
-//     most 2^-11 of each weight, half of what rounding the output adds; with 8
-//     rows the products are cheap enough to add the remainder as a second FP16
-//     term (HILO: 22 bits). At a piece's end the warps' states are joined through
+//     below 2^8 in FP16), O^T += V^T P^T. P is two FP16 terms, its rounding and the
+//     rounded rest (22 bits): one alone is off by 2^-11 of each weight, as much as
+//     rounding the output adds. At a piece's end the warps' states are joined through
 //     the stage just read, 8 RW rows at a time, and written as its partial.
 // Keys that do not count (past the end, or without a page) are masked in the
 // logits and in the V fragments, so what their staged rows hold does not matter.
@@ -56,10 +55,9 @@ struct SpanRec {  // one staged tile, producer -> math warps
 };
 constexpr int kSpanFirst = 1, kSpanLast = 2, kSpanEnd = 4;
 
-template <int D_, int NT_, int RW_, int STAGES_, bool HILO_>
+template <int D_, int NT_, int RW_, int STAGES_>
 struct SpanMma {
   static constexpr int D = D_, NT = NT_, RW = RW_, STAGES = STAGES_;
-  static constexpr bool HILO = HILO_;
   static constexpr int ROWS = 8 * NT * RW, TILE = D == 64 ? 128 : 64, UNITS = TILE / 16;
   static constexpr int KW = 4 / RW;           // warps that split a tile's keys
   static constexpr int KB = UNITS / KW;       // 16-key blocks per warp
@@ -470,10 +468,8 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
             sc[sb][i][2 * e2 + 1] = w1r;
             const uint32_t hi = pack_half2(w0r, w1r);
             bh[sb][i][e2] = movmatrix_t(hi);
-            if constexpr (C::HILO) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-              bl[sb][i][e2] = movmatrix_t(pack_half2(w0r - f.x, w1r - f.y));
-            }
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            bl[sb][i][e2] = movmatrix_t(pack_half2(w0r - f.x, w1r - f.y));
           }
       }
       if (causal) {
@@ -538,11 +534,9 @@ prefix_span_kernel(const PrefixParams p, const SpanSet ss, const __grid_constant
 #pragma unroll
             for (int i = 0; i < NT; ++i)
               mma_16816(acc[k][i], a0, a1, a2, a3, bh[sb][i][0], bh[sb][i][1]);
-            if constexpr (C::HILO) {
 #pragma unroll
-              for (int i = 0; i < NT; ++i)
-                mma_16816(acc[k][i], a0, a1, a2, a3, bl[sb][i][0], bl[sb][i][1]);
-            }
+            for (int i = 0; i < NT; ++i)
+              mma_16816(acc[k][i], a0, a1, a2, a3, bl[sb][i][0], bl[sb][i][1]);
           }
         }
       }

@@ -14,7 +14,7 @@
 //   * warps 0-3 and 4-7: softmax of query tile 0 and 1, one row per thread: read
 //     the S row from TMEM, base-2 softmax against a running maximum that is
 //     raised only when a logit passes it by 2^8 (O in TMEM is rescaled then;
-//     exact after the final division), write P as FP16 over half of S in TMEM.
+//     exact after the final division), write P in two FP16 terms over S in TMEM.
 //   * warps 9 and 10: TMA, for K and for V (one warp issues a 16-row box every
 //     ~100 cycles, the TMA unit takes one every 61). K and V tiles (128 keys) go
 //     through one ring of buffers in the order K0 V0 K1 V1 ..
@@ -24,16 +24,18 @@
 //     The MMAs of a CTA run in issue order, so S_{j+1} may overwrite P_j
 //     without a barrier, and the commit that publishes S_{j+1} also says that
 //     O holds P_j V_j (what a rescale needs).
-// Measured on 4096 rows x 8192 keys x 8 heads: 1.14 PFLOP/s. 64-key tiles with two S
-// buffers per query tile, with one or two issuing warps, and two threads per row
-// were no faster (128 and 130 us against 120), two threads per row on 128-key
-// tiles slower (they spill).
+// Measured on 4096 rows x 8192 keys x 8 heads, 128 dims: 168 us, 0.82 PFLOP/s of the formula's
+// operations and half as many again for the second term of P (137 us without it).
+// Handing P over in halves (the product of one while the other is exponentiated) or
+// reading the logits a quarter ahead were slower (190 to 200 against 178 with the join), as was
+// rounding the first term and converting it back (190).
 // TMEM: S0 S1 O0 O1, 128 columns each = all 512.
 // Query rows: a tile holds floor(128 / G) tokens with all G heads of the kv
 // head, one TMA box {64 columns, G heads, floor(128 / G) tokens}, so any group
 // size fills the tile up to its remainder.
-// Bound: the tensor cores (4 x 512 cycles per two row tiles and key tile) and
-// the exponentials (2 x 128 x 128 at 16 a cycle = 2048 cycles) alike.
+// Bound: a row tile's chain of softmax (128 exponentials and their two terms per thread),
+// P V and the next Q K^T, two of which overlap. The tensor cores alone take 6 x 512 cycles
+// per two row tiles and key tile, the exponentials 2 x 128 x 128 at 16 a cycle = 2048.
 #pragma once
 
 #include "shared_prefix_mma.cuh"
@@ -89,17 +91,26 @@ __device__ __forceinline__ float max64(const uint32_t* s) {
   for (int y = 0; y < 8; ++y) mx[y] = fmaxf(mx[y], __uint_as_float(s[56 + y]));
   return fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
 }
-// pk = 2^(c s - ref) as FP16 pairs; returns their FP32 sum (of the unrounded weights).
+// The weights 2^(c s - ref) of 64 keys in two FP16 terms, as pairs: of each 32 keys
+// pk[0 .. 15] the first 11 bits (cut off, so that the rest is exact), pk[16 .. 31] the rest,
+// rounded to 11 bits. Together 2^-21 of a weight is lost at most (2^-25 in all below
+// 2^-14, where FP16 thins out; a row's largest weight is 1 at least). One rounded FP16 number
+// is off by 2^-11 of a weight, as much as rounding the output adds. Returns the weights' sum in FP32.
 __device__ __forceinline__ float weights64(const uint32_t* s, uint32_t* pk, float c, float ref) {
-  const uint64_t c2 = f2(c, c), nm2 = f2(-ref, -ref);
+  const uint64_t c2 = f2(c, c), nm2 = f2(-ref, -ref), minus = f2(-1.f, -1.f);
   uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
   for (int x = 0; x < 32; ++x) {
     float y0, y1;
     f2_split(ffma2(f2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), c2, nm2), y0, y1);
     const float a = ex2(y0), b = ex2(y1);
-    sum[x & 3] = fadd2(sum[x & 3], f2(a, b));
-    pk[x] = pack_half2(a, b);
+    const uint64_t w = f2(a, b);
+    sum[x & 3] = fadd2(sum[x & 3], w);
+    const float ah = __uint_as_float(__float_as_uint(a) & 0xffffe000u);
+    const float bh = __uint_as_float(__float_as_uint(b) & 0xffffe000u);
+    pk[(x & 16) + x] = pack_half2(ah, bh);
+    f2_split(ffma2(f2(ah, bh), minus, w), y0, y1);
+    pk[(x & 16) + 16 + x] = pack_half2(y0, y1);
   }
   float r[8];
 #pragma unroll
@@ -296,10 +307,13 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
           __syncwarp();
           tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            tc_mma_ts_elect(tmem + C::O_COL + i * 128, tmem + C::S_COL + i * 128 + 64 + kk * 8,
-                            v_desc + vb * STEP + kk * (16 * 128 >> 4), IDESC_O,
-                            (j > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < BN / 16; ++kk)  // 16 keys: both terms of P
+#pragma unroll
+            for (int term = 0; term < 2; ++term)
+              tc_mma_ts_elect(tmem + C::O_COL + i * 128,
+                              tmem + C::S_COL + i * 128 + (kk >> 1) * 32 + term * 16 + (kk & 1) * 8,
+                              v_desc + vb * STEP + kk * (16 * 128 >> 4), IDESC_O,
+                              (j > 0 || kk + term > 0) ? 1u : 0u);
           if (!more) tc_commit_elect(&o_full[i]);
           if (i == nt - 1) tc_commit_elect(&empty[vb]);
           if (more) {
@@ -360,11 +374,14 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
           }
           // all logits -inf so far: any finite reference gives weights 0
           const float ref = m_used == -INFINITY ? 0.f : m_used;
-          // Pass 2: weights, second half first; P goes to columns 64 .. 127, whose
-          // logits are in registers by then.
-          uint32_t pk[32];
+          // Pass 2: weights, second half first, the two terms of 32 keys over their own
+          // logits (which are in registers by then).
+          uint32_t pk[64];
           float sum = weights64(s, pk, c, ref);
-          if (real) tc_st32(s_col + 96, pk);
+          if (real) {
+            tc_st32(s_col + 64, pk);
+            tc_st32(s_col + 96, pk + 32);
+          }
           tc_ld32(s_col, s);
           tc_ld32(s_col + 32, s + 32);
           tc_wait_ld();
@@ -378,7 +395,8 @@ prefix_tc_kernel(const PrefixTcParams p, const __grid_constant__ CUtensorMap qma
             l = 0.f;
             continue;
           }
-          tc_st32(s_col + 64, pk);
+          tc_st32(s_col, pk);
+          tc_st32(s_col + 32, pk + 32);
           if (valid < BN && i == 0) {
             // V rows past the prefix (stale cells of its last unit): zeros. K and V
             // alternate in the ring: this tile's V is buffer 2 * tile + 1.

@@ -1,0 +1,47 @@
+"""The serving operators where their kernels could lose bits, marks or order:
+weights between two FP16 numbers, values that are not finite, calls from several
+threads, launches past a grid's limits, paths that only large calls take.
+
+Each bound is derived at its test; inputs and calls as in test_gpu_serving_ops.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import serving_oracle as oracle
+from test_gpu_serving_ops import IMPLS, call, impl_of, make
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- the weights' precision ----------------------------------------------------
+@pytest.mark.parametrize("impl", IMPLS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 3, 6, 16])
+def test_weights_keep_more_than_sixteen_bits(pkg, cuda, T, D, impl):
+    # Half of the keys have weight 1 and value 1, half a weight w in (0.5, 0.53) and
+    # a value near -1 / w: the outputs are small, so that FP16 rounds them by
+    # 2^-11 of little, and an error of the weights shows. One FP16 number per weight
+    # is off by up to 2^-12, 3e-4 of an output. Allowed beside the output's rounding:
+    # two FP16 terms 2^-21, the exponential 2^-22 and the logit 2^-23 of a weight
+    # (1e-6, times values of 2), sums of 500 terms in FP32 1.5e-6.
+    B, G, KVH, prefix = 12, 4, 2, 200
+    lengths = [T + 21 * b for b in range(B)]
+    d = make(B, T, G * KVH, KVH, D, torch.float16, prefix, lengths)
+    g = torch.Generator().manual_seed(9)
+    d["q"].zero_()
+    d["q"][..., 0] = (torch.rand(B, T, G * KVH, generator=g) * 0.05 + 0.64) * D ** 0.5 / 2  # ln 2 = 0.693
+    used = [(d["prefix_table"], prefix)] + [(d["tables"][b], n) for b, n in enumerate(lengths)]
+    for table, n in used:
+        for t in range(n):
+            at = int(table[t // 16]), t % 16
+            d["k"][at], d["v"][at] = 0.0, 1.0
+            if t % 2:
+                d["k"][at][:, 0] = -2.0
+                d["v"][at] = -(torch.rand(KVH, D, generator=g) * 0.1 + 1.88).half()
+    got = call(pkg, d, cuda, impl).cpu().double()
+    want, _ = oracle.shared_prefix_attention(d["q"], d["k"], d["v"], d["prefix_table"], prefix,
+                                             d["tables"], d["lengths"])
+    over = (got - want).abs() - want.abs() * 2.0 ** -11
+    assert over.max().item() <= 4e-6
