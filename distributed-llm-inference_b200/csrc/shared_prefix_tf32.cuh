@@ -127,6 +127,7 @@ prefix_tf32_kernel(const PrefixParams p, int prefix_tiles, int own_tiles) {
   int page = page_of(k0 + KT);
   for (int i = tid; i < RT; i += C::NT) redo[i] = 0;
   if (tid == 0) *odd_key = INT_MAX;
+  __syncthreads();  // before any thread marks a key
   int row[2], limit[2];  // rows of the item; keys [0, limit) are seen
 #pragma unroll
   for (int e = 0; e < 2; ++e) {

@@ -45,3 +45,36 @@ def test_weights_keep_more_than_sixteen_bits(pkg, cuda, T, D, impl):
                                              d["tables"], d["lengths"])
     over = (got - want).abs() - want.abs() * 2.0 ** -11
     assert over.max().item() <= 4e-6
+
+
+# ---- values that are not finite ------------------------------------------------
+def poison(d, b, token, dim, value, what="v"):
+    """One dim of own token `token` of sequence b, every kv head."""
+    d[what][int(d["tables"][b, token // 16]), token % 16, :, dim] = value
+
+
+@pytest.mark.parametrize("impl", ["auto", "simt"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [2, 4, 7, 10, 20])
+def test_a_drafted_value_that_is_not_finite(pkg, cuda, T, D, impl):
+    # V alone (the logits stay finite): the rows that see the token get it, the others
+    # keep their bits. Drafted tokens in the first tile of a key range, in the
+    # first, and in a later range; 4 T rows per kv head.
+    lengths = [T, T + 3, T + 30, T + 140, T + 411]
+    d = make(len(lengths), T, 8, 2, D, torch.float32, 30, lengths)
+    clean = call(pkg, d, cuda, impl).cpu()
+    for first in (T - 1, T // 2):  # the rows from this one on see the token
+        e = dict(d, v=d["v"].clone())
+        for b, n in enumerate(lengths):
+            poison(e, b, n - T + first, 3, float("inf"))
+            poison(e, b, n - T + first, 5, float("nan"))
+        for _ in range(5):
+            got = call(pkg, e, cuda, impl).cpu()
+            assert torch.equal(got[:, :first], clean[:, :first])
+            assert (got[:, first:, :, 3] == float("inf")).all()
+            assert got[:, first:, :, 5].isnan().all()
+            keep = [i for i in range(D) if i not in (3, 5)]
+            # the same sums in another order and arithmetic: twice the bound of one result
+            top = d["v"][d["v"] == d["v"]].abs().max().item()
+            assert (got[..., keep] - clean[..., keep]).abs().max().item() <= 4e-5 * top
+    assert pkg.read_device_errors() == 0
