@@ -476,8 +476,15 @@ int check_attention_args(int64_t B, int64_t H, int64_t D, int64_t N, int64_t bs,
   return PDB_OK;
 }
 
+// Binds the device's context to a thread that has made no runtime call yet that
+// does: encoding a tensor map is a driver call, which fails without one.
 int current_device(int* dev) {
+  thread_local int bound = -1;
   cudaError_t e = cudaGetDevice(dev);
+  if (e == cudaSuccess && *dev != bound) {
+    e = cudaSetDevice(*dev);
+    if (e == cudaSuccess) bound = *dev;
+  }
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   return PDB_OK;
 }
@@ -1017,8 +1024,8 @@ int pdb_prefill_attention_impl(const void* q, const void* k_pool, const void* v_
                     : "the tcgen05 prefill kernel needs under 2^31 pool rows and query rows");
   const bool use_tc = impl == PDB_PREFILL_TCGEN05 || (impl == PDB_PREFILL_AUTO && tc_ok);
   int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (const int rc = current_device(&dev)) return rc;
+  cudaError_t e = cudaSuccess;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int G = (int)(heads / kv_heads);
   const int bs_shift = ((block_size & (block_size - 1)) == 0)

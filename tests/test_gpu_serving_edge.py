@@ -6,6 +6,8 @@ Each bound is derived at its test; inputs and calls as in test_gpu_serving_ops.
 """
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -13,6 +15,52 @@ import serving_oracle as oracle
 from test_gpu_serving_ops import IMPLS, call, impl_of, make
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- calls from several threads ------------------------------------------------
+def in_threads(jobs):
+    """Runs the callables at the same time; raises what any of them raised."""
+    errors = []
+
+    def guarded(job):
+        try:
+            job()
+        except BaseException as e:  # noqa: BLE001 - handed to the caller
+            errors.append(e)
+    threads = [threading.Thread(target=guarded, args=(j,)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if errors:
+        raise errors[0]
+
+
+@pytest.mark.parametrize("op", ["mma", "tcgen05", "decode", "prefill"])
+def test_first_call_of_a_thread(pkg, cuda, op):
+    # a new thread has no CUDA context bound: encoding tensor maps needs one
+    d = make(3, 2, 8, 2, 64, torch.float16, 30, [4, 20, 67], stale=0.0)
+    c = {n: t.to(cuda) if isinstance(t, torch.Tensor) else t for n, t in d.items()}
+    one, out = c["q"][:, 0].contiguous(), torch.empty_like(c["q"])
+    first = torch.empty_like(one)
+
+    def job():
+        if op == "decode":
+            pkg.paged_attention(one, c["k"], c["v"], c["tables"], c["lengths"], 67, out=first)
+        elif op == "prefill":
+            pkg.prefill_attention(c["q"], c["k"], c["v"], c["tables"],
+                                  c["lengths"].clamp(max=2), out=out)
+        else:
+            pkg.shared_prefix_attention(c["q"], c["k"], c["v"], c["prefix_table"], 30, c["tables"],
+                                        c["lengths"], 67, out=out, impl=impl_of(pkg, op))
+    job()
+    torch.cuda.synchronize()
+    want = [first.clone(), out.clone()]
+    first.zero_(), out.zero_()
+    in_threads([job])
+    torch.cuda.synchronize()
+    assert torch.equal(first, want[0] if op == "decode" else torch.zeros_like(first))
+    assert torch.equal(out, torch.zeros_like(out) if op == "decode" else want[1])
 
 
 # ---- the weights' precision ----------------------------------------------------
