@@ -60,6 +60,17 @@ def workspace(device: torch.device, stream: int, nbytes: int, tag: str) -> torch
         return buf
 
 
+# A call that makes several launches over its workspace holds this lock while it issues
+# them: another thread's launches on the same stream (the C call runs without the
+# interpreter lock) would come between them and overwrite the scratch they share.
+_launch_locks: dict[tuple[int, int, str], threading.Lock] = {}
+
+
+def launch_lock(device: int, stream: int, tag: str) -> threading.Lock:
+    key = (device, stream, tag)
+    return _launch_locks.get(key) or _launch_locks.setdefault(key, threading.Lock())
+
+
 # The current stream's handle without building a torch.cuda.Stream (2 us a call).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -133,12 +144,13 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tables: t
     with _DeviceGuard(q.device):
         stream = _stream_ptr(q.device)
         need = lib.pdb_paged_attention_workspace_size(B, H, KVH, D, int(max_length), dt)
-        ws = workspace(q.device, stream, need, "attention")
-        rc = lib.pdb_paged_attention_impl(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
-            out.data_ptr(), B, H, D, N, bs, KVH, Dk, tables.size(1), int(max_length), dt,
-            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-            stream, int(impl))
+        with launch_lock(q.device.index, stream, "attention"):
+            ws = workspace(q.device, stream, need, "attention")
+            rc = lib.pdb_paged_attention_impl(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
+                out.data_ptr(), B, H, D, N, bs, KVH, Dk, tables.size(1), int(max_length), dt,
+                ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                stream, int(impl))
     _lib.check(rc, "paged_attention")
     return out
 
@@ -204,15 +216,16 @@ def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pool: tor
     with _DeviceGuard(q.device):
         stream = _stream_ptr(q.device)
         need = lib.pdb_rope_kv_write_workspace_size(B, S, 1 if valid is not None else 0)
-        ws = workspace(q.device, stream, need, "rope")
-        rc = lib.pdb_rope_kv_write(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
-            k_pool.data_ptr(), v_pool.data_ptr(), pos.data_ptr(), sb, ss, inv_freq.data_ptr(),
-            physical.data_ptr(), offsets.data_ptr(), physical.numel(),
-            valid.data_ptr() if valid is not None else None, B, S, H, KVH, D,
-            k_pool.size(0), k_pool.size(1), _DTYPES[q.dtype],
-            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-            stream)
+        with launch_lock(q.device.index, stream, "rope"):
+            ws = workspace(q.device, stream, need, "rope")
+            rc = lib.pdb_rope_kv_write(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
+                k_pool.data_ptr(), v_pool.data_ptr(), pos.data_ptr(), sb, ss, inv_freq.data_ptr(),
+                physical.data_ptr(), offsets.data_ptr(), physical.numel(),
+                valid.data_ptr() if valid is not None else None, B, S, H, KVH, D,
+                k_pool.size(0), k_pool.size(1), _DTYPES[q.dtype],
+                ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                stream)
     _lib.check(rc, "rope_kv_write")
     if squeeze:
         return q_out.squeeze(1), k_out.squeeze(1)

@@ -16,7 +16,7 @@ import functools
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _DeviceGuard, _stream_ptr, workspace
+from .ops import _DTYPES, _DeviceGuard, _stream_ptr, launch_lock, workspace
 
 _INT32, _INT64, _FP32 = torch.int32, torch.int64, torch.float32
 _current_device = torch.cuda.current_device
@@ -144,13 +144,14 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         stream = _stream_ptr(where)
         need = _prefix_workspace(device, B, T, H, KVH, D, prefix_length, max_length, dt,
                                  width > 0)
-        ws = workspace(where, stream, need, "shared_prefix")
-        return _lib.load().pdb_shared_prefix_attention_impl(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), prefix_table.data_ptr(), pages,
-            prefix_length, tables.data_ptr(), lengths.data_ptr(),
-            counts.data_ptr() if counts is not None else None, scores_ptr, scores_out_ptr, width,
-            out.data_ptr(), B, T, H, D, N, bs, KVH, table_width, max_length, dt,
-            ws.data_ptr() if ws is not None else None, need, stream, impl)
+        with launch_lock(device, stream, "shared_prefix"):
+            ws = workspace(where, stream, need, "shared_prefix")
+            return _lib.load().pdb_shared_prefix_attention_impl(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), prefix_table.data_ptr(), pages,
+                prefix_length, tables.data_ptr(), lengths.data_ptr(),
+                counts.data_ptr() if counts is not None else None, scores_ptr, scores_out_ptr,
+                width, out.data_ptr(), B, T, H, D, N, bs, KVH, table_width, max_length, dt,
+                ws.data_ptr() if ws is not None else None, need, stream, impl)
 
     _run_on(device, launch, "shared_prefix_attention")
     return out if scores is None else (out, scores_out)

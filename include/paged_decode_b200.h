@@ -394,7 +394,9 @@ PDB_API int64_t pdb_fast_grid_size(int64_t batch, int64_t heads, int64_t kv_head
  * Lengths and counts out of range are clamped, pages out of range read as
  * zeros; both set device error bits. Results do not depend on timing.
  * Capturable. The workspace is 256-byte aligned, of
- * pdb_shared_prefix_attention_workspace_size bytes; contents do not matter.
+ * pdb_shared_prefix_attention_workspace_size bytes; contents do not matter. A call is
+ * several launches: no other call may use the same workspace from another
+ * thread while it is being issued, nor from another stream while it runs.
  */
 PDB_API int pdb_shared_prefix_attention(
     const void* q, const void* k_pool, const void* v_pool, const int32_t* prefix_table,

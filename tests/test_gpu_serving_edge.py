@@ -7,11 +7,13 @@ Each bound is derived at its test; inputs and calls as in test_gpu_serving_ops.
 from __future__ import annotations
 
 import threading
+import time
 
 import pytest
 import torch
 
 import serving_oracle as oracle
+from conftest import import_module
 from test_gpu_serving_ops import IMPLS, call, impl_of, make
 
 pytestmark = pytest.mark.gpu
@@ -126,3 +128,58 @@ def test_a_drafted_value_that_is_not_finite(pkg, cuda, T, D, impl):
             top = d["v"][d["v"] == d["v"]].abs().max().item()
             assert (got[..., keep] - clean[..., keep]).abs().max().item() <= 4e-5 * top
     assert pkg.read_device_errors() == 0
+
+
+# ---- scratch that calls share ------------------------------------------------------
+def test_a_call_is_issued_whole(pkg, cuda, monkeypatch):
+    # a library that launches nothing and says when two calls of one stream overlap
+    lib, state = import_module("_lib"), dict(inside=0, overlapped=False, calls=0)
+    real = lib.load()
+
+    class Quiet:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def issue(self, *args):
+            state["inside"] += 1
+            state["overlapped"] |= state["inside"] > 1
+            time.sleep(0.02)
+            state["inside"] -= 1
+            state["calls"] += 1
+            return 0
+        pdb_shared_prefix_attention_impl = pdb_rope_kv_write = pdb_paged_attention_impl = issue
+
+    d = make(3, 2, 8, 2, 64, torch.float16, 30, [4, 20, 67])
+    quiet = Quiet()
+    monkeypatch.setattr(lib, "load", lambda: quiet)
+    q = torch.zeros(3, 8, 64, dtype=torch.float16, device=cuda)
+    pool = torch.zeros(8, 16, 2, 64, dtype=torch.float16, device=cuda)
+    ints = torch.zeros(3, 4, dtype=torch.int32, device=cuda)
+    long = torch.zeros(3, dtype=torch.long, device=cuda)
+    inv_freq, kv = torch.ones(32, device=cuda), torch.zeros_like(q[:, :2].contiguous())
+    for job in (lambda: call(pkg, d, cuda),
+                lambda: pkg.paged_attention(q, pool, pool, ints, ints[:, 0].contiguous(), 64),
+                lambda: pkg.rope_kv_write(q, kv, kv, pool, pool, long, long, long[:, None], inv_freq)):
+        state.update(inside=0, overlapped=False, calls=0)
+        in_threads([job] * 4)
+        assert state["calls"] == 4 and not state["overlapped"]
+
+
+def test_threads_that_share_a_stream(pkg, cuda):
+    jobs = [make(20, 3, 8, 2, 64, dtype, 300, [5 + 3 * i for i in range(20)], seed=s, scores=True)
+            for s, dtype in enumerate([torch.float16, torch.float16, torch.float32])]
+    alone = [call(pkg, d, cuda) for d in jobs]
+    inputs = [{n: t.to(cuda) if isinstance(t, torch.Tensor) else t for n, t in d.items()} for d in jobs]
+    torch.cuda.synchronize()
+    got = [[] for _ in jobs]
+
+    def repeat(c, results):
+        for _ in range(60):
+            results.append(pkg.shared_prefix_attention(
+                c["q"], c["k"], c["v"], c["prefix_table"], c["prefix"], c["tables"], c["lengths"],
+                c["max_length"], scores=c["scores"], scores_out=torch.empty_like(c["scores"])))
+    in_threads([lambda c=c, r=r: repeat(c, r) for c, r in zip(inputs, got)])
+    torch.cuda.synchronize()
+    for want, results in zip(alone, got):
+        assert len(results) == 60
+        assert all(torch.equal(x, want[0]) and torch.equal(y, want[1]) for x, y in results)
