@@ -429,7 +429,9 @@ int pdb_shared_prefix_attention_impl(
     return fail(PDB_ERR_INVALID_ARGUMENT, "give both scores and their output");
   if (scores && scores_width < max_length)
     return fail(PDB_ERR_INVALID_ARGUMENT, "scores must hold max_length tokens");
-  if (scores && scores_width > INT32_MAX) return fail(PDB_ERR_INVALID_ARGUMENT, "shape too large");
+  if (scores && (scores_width > INT32_MAX ||
+                 (scores_width + 1023) / 1024 > INT32_MAX / (batch * kv_heads)))
+    return fail(PDB_ERR_INVALID_ARGUMENT, "shape too large");
   if (impl < PDB_PREFIX_AUTO || impl > PDB_PREFIX_TCGEN05)
     return fail(PDB_ERR_INVALID_ARGUMENT, "unknown kernel selection");
   if (!q || !k_pool || !v_pool || !lengths || !out || (prefix_length > 0 && !prefix_table) ||
@@ -516,8 +518,8 @@ int pdb_shared_prefix_attention_impl(
   }
   if (e == cudaSuccess && scores && scores_width > 0)
     e = launch_pdl(pdb::prefix_scores_kernel,
-                   dim3((unsigned)((scores_width + 1023) / 1024), (unsigned)(p.B * p.KVH)),
-                   dim3(256), 0, st, p);
+                   dim3((unsigned)((scores_width + 1023) / 1024 * p.B * p.KVH)), dim3(256), 0, st,
+                   p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "shared prefix attention launch");
   return PDB_OK;

@@ -771,21 +771,22 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
 __global__ void __launch_bounds__(256) prefix_scores_kernel(const PrefixParams p) {
   grid_dependency_wait();
   launch_dependents();
-  const int64_t bh = blockIdx.y;
-  const int b = (int)(bh / p.KVH), h = (int)(bh - (int64_t)b * p.KVH);
-  const int j0 = blockIdx.x * 1024 + threadIdx.x, TG = p.T * p.G;
+  const int per = (int)((p.scores_width + 1023) / 1024), bh = blockIdx.x / per;
+  const int b = bh / p.KVH, h = bh - b * p.KVH;
+  const int64_t j0 = (int64_t)(blockIdx.x - bh * per) * 1024 + threadIdx.x;
+  const int TG = p.T * p.G;
   constexpr int U = 4;
-  const float* in = p.scores + bh * p.scores_width;
+  const float* in = p.scores + (int64_t)bh * p.scores_width;
   float old[U], add[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int j = j0 + 256 * u;
+    const int64_t j = j0 + 256 * u;
     old[u] = j < p.scores_width ? in[j] : 0.f;
     add[u] = 0.f;
   }
   int n, count;
   prefix_sequence(p, b, n, count);
-  const float* lg = p.logits + bh * p.logits_width * TG;
+  const float* lg = p.logits + (int64_t)bh * p.logits_width * TG;
   if (j0 < n) {
     for (int t = 0; t < count; ++t) {
       const int limit = prefix_limit(n, count, t);
@@ -796,8 +797,8 @@ __global__ void __launch_bounds__(256) prefix_scores_kernel(const PrefixParams p
         const bool wide = (TG & 3) == 0 && here == 4 && (p.G & 3) == 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int j = j0 + 256 * u;
-          const float* src = lg + (int64_t)j * TG + t * p.G + g;
+          const int64_t j = j0 + 256 * u;
+          const float* src = lg + j * TG + t * p.G + g;
           if (wide) {
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
             if (j < limit) y = *reinterpret_cast<const float4*>(src);
@@ -820,8 +821,8 @@ __global__ void __launch_bounds__(256) prefix_scores_kernel(const PrefixParams p
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int j = j0 + 256 * u;
-    if (j < p.scores_width) p.scores_out[bh * p.scores_width + j] = old[u] + add[u];
+    const int64_t j = j0 + 256 * u;
+    if (j < p.scores_width) p.scores_out[(int64_t)bh * p.scores_width + j] = old[u] + add[u];
   }
 }
 

@@ -414,3 +414,10 @@ def test_evict_tokens_argument_checks(lib, kw, msg):
                                 a["D"], a["N"], a["bs"], a["KVH"], a["W"], a["W2"], a["budget"],
                                 a["recent"], a["dtype"], None) == 1
     assert _lib.last_error() == msg
+
+
+def test_scores_of_more_blocks_than_a_grid_holds_are_refused(lib):
+    # before anything is launched, like every other refusal
+    kw = dict(scores=64, scores_out=64, width=1 << 30, B=60000, KVH=2, H=2, T=1)
+    assert prefix_attn(lib, **kw) == 1
+    assert _lib.last_error() == "shape too large"

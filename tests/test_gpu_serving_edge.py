@@ -14,7 +14,7 @@ import torch
 
 import serving_oracle as oracle
 from conftest import import_module
-from test_gpu_serving_ops import IMPLS, call, impl_of, make
+from test_gpu_serving_ops import IMPLS, TOL, call, impl_of, make
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +183,27 @@ def test_threads_that_share_a_stream(pkg, cuda):
     for want, results in zip(alone, got):
         assert len(results) == 60
         assert all(torch.equal(x, want[0]) and torch.equal(y, want[1]) for x, y in results)
+
+
+# ---- sizes past a limit of the launch -------------------------------------------
+def test_accumulated_weights_of_very_many_heads(pkg, cuda):
+    # batch x kv heads above 65535; the sequences share a few pages, which are read only
+    B, H, KVH, D, width = 8200, 16, 8, 64, 24
+    g = torch.Generator().manual_seed(4)
+    d = make(1, 1, H, KVH, D, torch.float16, 20, [16 * 40])
+    d.update(q=torch.randn(B, 1, H, D, generator=g).half(), max_length=width,
+             tables=d["tables"][0][torch.randint(0, 40, (B, 2), generator=g)],
+             lengths=torch.randint(0, width + 1, (B,), generator=g).to(torch.int32),
+             scores=torch.rand(B, KVH, width + 5, generator=g))
+    out, scores = call(pkg, d, cuda)
+    some = [0, 1, 4095, 4096, 8190, 8191, 8192, 8199]
+    want, want_scores = oracle.shared_prefix_attention(
+        d["q"][some], d["k"], d["v"], d["prefix_table"], 20, d["tables"][some], d["lengths"][some],
+        None, d["scores"][some])
+    top = d["v"][d["v"] == d["v"]].abs().max().item()
+    assert (out.cpu()[some].double() - want).abs().max().item() <= TOL[torch.float16] * top
+    torch.testing.assert_close(scores.cpu()[some].double(), want_scores, rtol=2e-5, atol=2e-6)
+    for part in (slice(0, 4100), slice(4100, B)):  # the same in two calls
+        _, half = call(pkg, dict(d, **{n: d[n][part] for n in ("q", "tables", "lengths", "scores")}), cuda)
+        torch.testing.assert_close(scores[part], half, rtol=4e-5, atol=4e-6)
+    assert pkg.read_device_errors() == 0
