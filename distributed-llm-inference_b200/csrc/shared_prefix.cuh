@@ -626,6 +626,46 @@ __device__ __forceinline__ PartRange prefix_parts(const PartSet& s, int seg, int
   return PartRange{(int64_t)(seg + c.x) * s.R + lr, s.R, c.y - c.x + 1};
 }
 
+// sum 2^(s_j - m) v_j of one row in plain FP32, key by key, four dims per lane and LPR lanes
+// of a warp (`mask`): for rows whose sum came out as a NaN although their logits have none. The
+// tensor cores take a weight as two FP16 numbers, and where one of them is 0 (a weight that
+// is exact in FP16, or too small for it) an infinite v_j gives 0 * inf. Rare and slow; not inlined, so
+// that the join's own code stays short.
+template <int LPR>
+__device__ __noinline__ float4 prefix_row_plain(const PrefixParams& p, int64_t row, int b, int h,
+                                                int limit, float m, unsigned mask) {
+  const int lane = threadIdx.x % LPR, D = p.D;
+  const bool in = 4 * lane < D;
+  float q[4] = {}, acc[4] = {};
+  if (in)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      q[i] = __half2float(static_cast<const __half*>(p.q)[row * D + 4 * lane + i]) * p.scale_log2;
+  for (int set = 0; set < 2; ++set) {
+    const int32_t* table = set ? p.tables + (int64_t)b * p.table_width : p.prefix_table;
+    const int width = set ? p.table_width : (p.prefix_length + p.block_size - 1) / p.block_size;
+    const int keys = set ? limit : p.prefix_length;
+    for (int j = 0; j < keys; ++j) {
+      const int64_t cell = prefix_cell(p, table, width, j);
+      const int64_t at = (cell * p.KVH + h) * D + 4 * lane;
+      float s = 0.f, v[4] = {};
+      if (in && cell >= 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s = fmaf(q[i], __half2float(static_cast<const __half*>(p.k_pool)[at + i]), s);
+          v[i] = __half2float(static_cast<const __half*>(p.v_pool)[at + i]);
+        }
+#pragma unroll
+      for (int i = LPR / 2; i; i >>= 1) s += __shfl_xor_sync(mask, s, i, LPR);
+      const float w = exp2f(s - m);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (w != 0.f) acc[i] = fmaf(w, v[i], acc[i]);
+    }
+  }
+  return make_float4(acc[0], acc[1], acc[2], acc[3]);
+}
+
 // VEC: D % 4 == 0 and D <= 128, four dims per lane, LPR lanes per row (D / 4
 // rounded up to 16 or 32); else up to 8 strided dims per lane, 32 lanes. Lane i
 // takes the (m, l) of part i, so the reads of O wait for nothing but the parts'
@@ -634,7 +674,8 @@ __device__ __forceinline__ PartRange prefix_parts(const PartSet& s, int seg, int
 // number) execute twice the instructions (256 x 4 x 32 rows: 15 us more). Parts are visited in order, so the sum does not depend
 // on which CTA finished first.
 template <typename T, int LPR, bool VEC>
-__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) {
+__global__ void __launch_bounds__(256)
+prefix_join_kernel(const __grid_constant__ PrefixParams p) {
   grid_dependency_wait();
   launch_dependents();
   constexpr int NV = VEC ? 4 : 8;
@@ -737,6 +778,16 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixParams p) 
   }
 #pragma unroll
   for (int i = LPR / 2; i; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+  if constexpr (VEC && sizeof(T) == 2) {
+    bool odd = false;  // NaN in the sum alone (a NaN logit is in l too)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) odd |= acc[i] != acc[i];
+    const unsigned mask = LPR == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+    if (__ballot_sync(0xffffffffu, odd && real && l == l && l != 0.f) & mask) {
+      const float4 y = prefix_row_plain<LPR>(p, row, b, h, limit, m, mask);
+      acc[0] = y.x; acc[1] = y.y; acc[2] = y.z; acc[3] = y.w;
+    }
+  }
   if (!real) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
   T* out = static_cast<T*>(p.out) + (int64_t)row * D;

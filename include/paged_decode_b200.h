@@ -390,7 +390,9 @@ PDB_API int64_t pdb_fast_grid_size(int64_t batch, int64_t heads, int64_t kv_head
  *            head c, summed (unchanged for j >= lengths[b]). May be the same
  *            buffer. scores_width >= max_length.
  * Query head h reads kv head h / (heads / kv_heads); scale 1 / sqrt(head_dim).
- * FP16: products on tensor cores, sums and softmax statistics in FP32.
+ * FP16: products on tensor cores with the weights as two FP16 numbers each (2^-21
+ * of a weight is lost at most), sums and softmax statistics in FP32. Infinities and
+ * NaN in K or V reach the rows that see them as in FP32 arithmetic, and no others.
  * Lengths and counts out of range are clamped, pages out of range read as
  * zeros; both set device error bits. Results do not depend on timing.
  * Capturable. The workspace is 256-byte aligned, of

@@ -103,15 +103,16 @@ def poison(d, b, token, dim, value, what="v"):
     d[what][int(d["tables"][b, token // 16]), token % 16, :, dim] = value
 
 
-@pytest.mark.parametrize("impl", ["auto", "simt"])
+@pytest.mark.parametrize("dtype, impl", [(torch.float32, "auto"), (torch.float32, "simt")]
+                         + [(torch.float16, i) for i in IMPLS])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("T", [2, 4, 7, 10, 20])
-def test_a_drafted_value_that_is_not_finite(pkg, cuda, T, D, impl):
+def test_a_drafted_value_that_is_not_finite(pkg, cuda, T, D, dtype, impl):
     # V alone (the logits stay finite): the rows that see the token get it, the others
     # keep their bits. Drafted tokens in the first tile of a key range, in the
     # first, and in a later range; 4 T rows per kv head.
     lengths = [T, T + 3, T + 30, T + 140, T + 411]
-    d = make(len(lengths), T, 8, 2, D, torch.float32, 30, lengths)
+    d = make(len(lengths), T, 8, 2, D, dtype, 30, lengths)
     clean = call(pkg, d, cuda, impl).cpu()
     for first in (T - 1, T // 2):  # the rows from this one on see the token
         e = dict(d, v=d["v"].clone())
@@ -126,7 +127,36 @@ def test_a_drafted_value_that_is_not_finite(pkg, cuda, T, D, impl):
             keep = [i for i in range(D) if i not in (3, 5)]
             # the same sums in another order and arithmetic: twice the bound of one result
             top = d["v"][d["v"] == d["v"]].abs().max().item()
-            assert (got[..., keep] - clean[..., keep]).abs().max().item() <= 4e-5 * top
+            assert (got[..., keep] - clean[..., keep]).abs().max().item() <= 2 * TOL[dtype] * top
+    assert pkg.read_device_errors() == 0
+
+
+@pytest.mark.parametrize("impl", IMPLS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,H,KVH,B", [(1, 4, 2, 2), (3, 8, 1, 2), (7, 16, 1, 2), (2, 8, 2, 40), (1, 9, 3, 5)])
+def test_infinities_that_every_row_sees_fp16(pkg, cuda, T, H, KVH, B, D, impl):
+    # as in FP32 arithmetic: an infinite v goes into its own dim only, whether its weight is
+    # a few bits long, or far below FP16's range; a key whose logit is -inf has no weight
+    lengths = [T + 37 + b % 3 for b in range(B)]
+    d = make(B, T, H, KVH, D, torch.float16, 150, lengths)
+    d["q"][..., 1], d["q"][..., 2] = d["q"][..., 1].abs() + 0.5, 1.0
+    for where, table, keys in [("prefix", d["prefix_table"], (5, 40, 140))] + [
+            ("own", t, (0, 3, 34)) for t in d["tables"]]:
+        at = [(int(table[n // 16]), n % 16) for n in keys]
+        d["v"][at[0]][:, 3 if where == "prefix" else 7] = float("inf" if where == "prefix" else "-inf")
+        d["k"][at[1]][:, 1] = float("-inf")
+        d["v"][at[2]][:, 9 if where == "prefix" else 11] = float("inf")
+        d["k"][at[2]][:, 2] = -240.0  # a weight of 2^-30 (D 128) or 2^-43, of those near 1
+    d["v"][int(d["prefix_table"][0]), 7, :, 13] = float("nan")
+    out = call(pkg, d, cuda, impl).cpu()
+    ref, _ = oracle.shared_prefix_attention(d["q"], d["k"], d["v"], d["prefix_table"], 150,
+                                            d["tables"], d["lengths"])
+    for dim, value in ((3, "inf"), (7, "-inf"), (9, "inf"), (11, "inf")):
+        assert (out[..., dim] == float(value)).all(), dim
+    assert out[..., 13].isnan().all()
+    keep = [i for i in range(D) if i not in (3, 7, 9, 11, 13)]
+    top = d["v"][torch.isfinite(d["v"])].abs().max().item()
+    assert (out[..., keep].double() - ref[..., keep]).abs().max().item() <= TOL[out.dtype] * top
     assert pkg.read_device_errors() == 0
 
 
