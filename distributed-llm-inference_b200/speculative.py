@@ -6,7 +6,7 @@ once; each step scores every request's drafted tokens in one pass over the
 layers (``shared_prefix_attention``: the prefix's K and V are read once for the
 batch), accepts drafts against the model's probabilities (``verify_drafts``)
 and, when a request's own cache passes its budget, keeps its most attended
-tokens (``evict_tokens``, on the weights the attention accumulated). The
+tokens (``evict_tokens``, on the weights that the tokens which stayed gave them). The
 reference decodes one token per request and step over whole contexts.
 
 Cached keys carry RoPE at the position where their token was seen, so a cache
@@ -59,6 +59,11 @@ class PrefixBatch:
         """Appends each request's tokens (one or more, ragged) to its cache and
         returns the logits that follow them, float32 [B, T, vocab] (rows past a
         request's own count are meaningless)."""
+        return self._forward(token_lists)
+
+    def _forward(self, token_lists, queries: list | None = None) -> torch.Tensor:
+        """``score``; with ``queries`` each layer's rotated queries are added to that
+        list, and no weights to the scores."""
         runner, cache = self.runner, self.runner.cache
         counts = [len(tokens) for tokens in token_lists]
         B, T = len(self.ids), max(counts)
@@ -75,6 +80,7 @@ class PrefixBatch:
             self.seen[rid] += n
         tables, lengths, longest = cache.metadata(self.ids)
         real = torch.tensor(counts, dtype=torch.int32, device=runner.device)
+        scores = self.scores if queries is None else None
         x = runner.model.model.embed_tokens(rows.to(runner.device))
         for index, layer in enumerate(runner.model.model.layers):
             attn = layer.self_attn
@@ -87,12 +93,26 @@ class PrefixBatch:
                                  runner.inv_freq, valid=valid, inplace=True)
             context = shared_prefix_attention(
                 q, keys, values, self.prefix_table, self.prefix_length, tables, lengths, longest,
-                counts=real, scores=self.scores[index] if self.scores is not None else None)
-            if self.scores is not None:
+                counts=real, scores=scores[index] if scores is not None else None)
+            if scores is not None:
                 context = context[0]
+            if queries is not None:
+                queries.append(q)
             x = x + attn.o_proj(context.reshape(B, T, -1))
             x = x + layer.mlp(layer.post_attention_layernorm(x))
         return runner.model.lm_head(runner.model.model.norm(x)).float()
+
+    def _accumulate(self, queries, counts) -> None:
+        """Adds the weights that each request's first ``counts`` query rows give, now that
+        its cache ends with those tokens. The other rows were rejected drafts, whose
+        weights would rank tokens by a text that is not there."""
+        cache = self.runner.cache
+        tables, lengths, longest = cache.metadata(self.ids)
+        real = torch.tensor(counts, dtype=torch.int32, device=self.runner.device)
+        for index, q in enumerate(queries):
+            shared_prefix_attention(q, cache.keys[index], cache.values[index], self.prefix_table,
+                                    self.prefix_length, tables, lengths, longest, counts=real,
+                                    scores=self.scores[index])
 
     @torch.inference_mode()
     def step(self, last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs=None,
@@ -102,12 +122,15 @@ class PrefixBatch:
         ``accept_uniforms`` fp32 [B, T], ``sample_uniforms`` fp32 [B];
         ``draft_probs`` fp32 [B, T, vocab], or None for drafts that were not
         sampled. Returns the new tokens of each request (1 to T + 1 of them):
-        distributed as the model's own, however good the drafts are."""
+        distributed as the model's own over what is cached, however good the drafts
+        are. With a budget the attention runs a second time, over the tokens that
+        stayed, for the weights that eviction goes by."""
         cache, device = self.runner.cache, self.runner.device
         T = accept_uniforms.shape[1]
         before = [cache.lengths[rid] for rid in self.ids]
         seen = dict(self.seen)
-        logits = self.score([[a, *d] for a, d in zip(last_tokens, drafts)])
+        queries = [] if self.scores is not None else None
+        logits = self._forward([[a, *d] for a, d in zip(last_tokens, drafts)], queries)
         probs = torch.softmax(logits / temperature, -1)
         if probs.shape[1] < T + 1:
             probs = torch.nn.functional.pad(probs, (0, 0, 0, T + 1 - probs.shape[1]))
@@ -120,9 +143,8 @@ class PrefixBatch:
             # the last token and the accepted drafts stay cached; cells past them are free
             cache.lengths[rid] = before[b] + len(got)
             self.seen[rid] = seen[rid] + len(got)
-            if self.scores is not None:
-                self.scores[:, b, :, cache.lengths[rid]:] = 0.0
         if self.budget is not None:
+            self._accumulate(queries, [len(got) for got in new])
             self.evict([rid for rid in self.ids if cache.lengths[rid] > self.budget])
         return new
 
