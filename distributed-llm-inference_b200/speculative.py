@@ -15,6 +15,8 @@ counted apart from its cache length.
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from .ops import rope_kv_write
@@ -54,12 +56,27 @@ class PrefixBatch:
         for rid in [*self.ids, _PREFIX]:
             self.runner.cache.release(rid)
 
+    @contextlib.contextmanager
+    def _unchanged_by_failure(self):
+        """What fails inside (no memory, a refused argument) leaves the requests as they
+        were. Scores are replaced, never changed in place; cells past a request's
+        length may hold anything."""
+        cache, seen, scores = self.runner.cache, dict(self.seen), self.scores
+        lengths = {rid: cache.lengths[rid] for rid in self.ids}
+        try:
+            yield
+        except BaseException:
+            cache.lengths.update(lengths)
+            self.seen, self.scores = seen, scores
+            raise
+
     @torch.inference_mode()
     def score(self, token_lists) -> torch.Tensor:
         """Appends each request's tokens (one or more, ragged) to its cache and
         returns the logits that follow them, float32 [B, T, vocab] (rows past a
         request's own count are meaningless)."""
-        return self._forward(token_lists)
+        with self._unchanged_by_failure():
+            return self._forward(token_lists)
 
     def _forward(self, token_lists, queries: list | None = None) -> torch.Tensor:
         """``score``; with ``queries`` each layer's rotated queries are added to that
@@ -81,6 +98,7 @@ class PrefixBatch:
         tables, lengths, longest = cache.metadata(self.ids)
         real = torch.tensor(counts, dtype=torch.int32, device=runner.device)
         scores = self.scores if queries is None else None
+        new_scores = torch.empty_like(scores) if scores is not None else None
         x = runner.model.model.embed_tokens(rows.to(runner.device))
         for index, layer in enumerate(runner.model.model.layers):
             attn = layer.self_attn
@@ -93,14 +111,22 @@ class PrefixBatch:
                                  runner.inv_freq, valid=valid, inplace=True)
             context = shared_prefix_attention(
                 q, keys, values, self.prefix_table, self.prefix_length, tables, lengths, longest,
-                counts=real, scores=scores[index] if scores is not None else None)
+                counts=real, **self._scored(scores, new_scores, index))
             if scores is not None:
                 context = context[0]
             if queries is not None:
                 queries.append(q)
             x = x + attn.o_proj(context.reshape(B, T, -1))
             x = x + layer.mlp(layer.post_attention_layernorm(x))
+        if scores is not None:
+            self.scores = new_scores
         return runner.model.lm_head(runner.model.model.norm(x)).float()
+
+    @staticmethod
+    def _scored(scores, new_scores, index) -> dict:
+        if scores is None:
+            return {}
+        return dict(scores=scores[index], scores_out=new_scores[index])
 
     def _accumulate(self, queries, counts) -> None:
         """Adds the weights that each request's first ``counts`` query rows give, now that
@@ -109,10 +135,12 @@ class PrefixBatch:
         cache = self.runner.cache
         tables, lengths, longest = cache.metadata(self.ids)
         real = torch.tensor(counts, dtype=torch.int32, device=self.runner.device)
+        new_scores = torch.empty_like(self.scores)
         for index, q in enumerate(queries):
             shared_prefix_attention(q, cache.keys[index], cache.values[index], self.prefix_table,
                                     self.prefix_length, tables, lengths, longest, counts=real,
-                                    scores=self.scores[index])
+                                    **self._scored(self.scores, new_scores, index))
+        self.scores = new_scores
 
     @torch.inference_mode()
     def step(self, last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs=None,
@@ -125,6 +153,11 @@ class PrefixBatch:
         distributed as the model's own over what is cached, however good the drafts
         are. With a budget the attention runs a second time, over the tokens that
         stayed, for the weights that eviction goes by."""
+        with self._unchanged_by_failure():
+            return self._step(last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs,
+                              temperature)
+
+    def _step(self, last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs, temperature):
         cache, device = self.runner.cache, self.runner.device
         T = accept_uniforms.shape[1]
         before = [cache.lengths[rid] for rid in self.ids]
@@ -155,15 +188,22 @@ class PrefixBatch:
         ids = [rid for rid in ids if cache.reserve((rid, "kept"), self.max_own)]
         if not ids:  # nothing to cut, or no free pages: the caches stay as they are
             return
-        rows = torch.tensor([self.ids.index(rid) for rid in ids], device=self.scores.device)
-        tables, lengths, _ = cache.metadata(ids)
-        new_tables = torch.tensor([cache.tables[(rid, "kept")] for rid in ids], dtype=torch.int32,
-                                  device=tables.device)
-        for index in range(self.scores.shape[0]):
-            _, _, kept = evict_tokens(cache.keys[index], cache.values[index],
-                                      self.scores[index][rows], tables, lengths, new_tables,
-                                      self.budget, self.recent)
-            self.scores[index][rows] = kept
+        try:
+            rows = torch.tensor([self.ids.index(rid) for rid in ids], device=self.scores.device)
+            tables, lengths, _ = cache.metadata(ids)
+            new_tables = torch.tensor([cache.tables[(rid, "kept")] for rid in ids],
+                                      dtype=torch.int32, device=tables.device)
+            scores = self.scores.clone()
+            for index in range(scores.shape[0]):
+                _, _, kept = evict_tokens(cache.keys[index], cache.values[index],
+                                          scores[index][rows], tables, lengths, new_tables,
+                                          self.budget, self.recent)
+                scores[index][rows] = kept
+        except BaseException:
+            for rid in ids:
+                cache.release((rid, "kept"))
+            raise
+        self.scores = scores
         for rid in ids:
             length = min(cache.lengths[rid], self.budget)
             pages = cache.tables[(rid, "kept")]
