@@ -24,6 +24,11 @@ from .serving_ops import evict_tokens, shared_prefix_attention, verify_drafts
 
 _PREFIX = "shared prefix"
 
+# Bytes of scratch that one attention call may take, about (partial sums, and with scores
+# every row's logits over the own tokens, which grow with the square of a prompt):
+# longer runs of tokens are scored piece by piece. Each piece sees those before it in the cache.
+_SCRATCH = 512 << 20
+
 
 class PrefixBatch:
     """Requests ``ids`` that continue ``prefix`` (token ids), up to ``max_own``
@@ -76,17 +81,43 @@ class PrefixBatch:
         returns the logits that follow them, float32 [B, T, vocab] (rows past a
         request's own count are meaningless)."""
         with self._unchanged_by_failure():
-            return self._forward(token_lists)
+            return self._score(token_lists)
 
-    def _forward(self, token_lists, queries: list | None = None) -> torch.Tensor:
+    def _piece(self, longest: int, scored: bool) -> int:
+        """Tokens per request that one attention call takes."""
+        runner = self.runner
+        per_token = 4 * len(self.ids) * runner.heads * (2 * runner.head_dim
+                                                        + (longest if scored else 0))
+        return max(1, min(4096, _SCRATCH // per_token))  # 4096: the operator's own limit
+
+    def _score(self, token_lists, queries: list | None = None) -> torch.Tensor:
         """``score``; with ``queries`` each layer's rotated queries are added to that
         list, and no weights to the scores."""
+        lengths, counts = self.runner.cache.lengths, [len(tokens) for tokens in token_lists]
+        after = [lengths[rid] + n for rid, n in zip(self.ids, counts)]
+        if any(not n for n in counts) or max(after) > self.max_own:
+            raise ValueError("each request takes one token at least, and max_own cached in all")
+        T, size = max(counts), self._piece(max(after), queries is None and self.scores is not None)
+        if T <= size:
+            return self._forward(token_lists, queries)
+        logits, kept = None, []
+        for t0 in range(0, T, size):
+            piece, kept_here = [tokens[t0:t0 + size] for tokens in token_lists], []
+            part = self._forward(piece, None if queries is None else kept_here)
+            if logits is None:
+                logits = part.new_empty((part.shape[0], T, part.shape[2]))
+            logits[:, t0:t0 + size] = part
+            kept.append(kept_here)
+        if queries is not None:
+            queries += [torch.cat(parts, 1) for parts in zip(*kept)]
+        return logits
+
+    def _forward(self, token_lists, queries: list | None) -> torch.Tensor:
+        """One pass over the layers; requests may have no token in it."""
         runner, cache = self.runner, self.runner.cache
         counts = [len(tokens) for tokens in token_lists]
         B, T = len(self.ids), max(counts)
         before = [cache.lengths[rid] for rid in self.ids]
-        if any(not n for n in counts) or any(b + n > self.max_own for b, n in zip(before, counts)):
-            raise ValueError("each request takes one token at least, and max_own cached in all")
         rows = torch.tensor([list(t) + [0] * (T - len(t)) for t in token_lists])
         first = torch.tensor([self.prefix_length + self.seen[rid] for rid in self.ids])
         positions = (first[:, None] + torch.arange(T)).to(runner.device)
@@ -135,12 +166,17 @@ class PrefixBatch:
         cache = self.runner.cache
         tables, lengths, longest = cache.metadata(self.ids)
         real = torch.tensor(counts, dtype=torch.int32, device=self.runner.device)
-        new_scores = torch.empty_like(self.scores)
-        for index, q in enumerate(queries):
-            shared_prefix_attention(q, cache.keys[index], cache.values[index], self.prefix_table,
-                                    self.prefix_length, tables, lengths, longest, counts=real,
-                                    **self._scored(self.scores, new_scores, index))
-        self.scores = new_scores
+        T, size = queries[0].shape[1], self._piece(longest, True)
+        for t0 in range(0, T, size):
+            here = (real - t0).clamp(0, size)  # a request's rows of this piece, and its
+            ends = lengths - (real - t0 - here).clamp(min=0)  # length with them
+            new_scores = torch.empty_like(self.scores)
+            for index, q in enumerate(queries):
+                shared_prefix_attention(q[:, t0:t0 + size].contiguous(), cache.keys[index],
+                                        cache.values[index], self.prefix_table,
+                                        self.prefix_length, tables, ends, longest, counts=here,
+                                        **self._scored(self.scores, new_scores, index))
+            self.scores = new_scores
 
     @torch.inference_mode()
     def step(self, last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs=None,
@@ -163,7 +199,7 @@ class PrefixBatch:
         before = [cache.lengths[rid] for rid in self.ids]
         seen = dict(self.seen)
         queries = [] if self.scores is not None else None
-        logits = self._forward([[a, *d] for a, d in zip(last_tokens, drafts)], queries)
+        logits = self._score([[a, *d] for a, d in zip(last_tokens, drafts)], queries)
         probs = torch.softmax(logits / temperature, -1)
         if probs.shape[1] < T + 1:
             probs = torch.nn.functional.pad(probs, (0, 0, 0, T + 1 - probs.shape[1]))

@@ -417,7 +417,9 @@ PDB_API int pdb_shared_prefix_attention_impl(
     int64_t block_size, int64_t kv_heads, int64_t table_width, int64_t max_length, int dtype,
     void* workspace, size_t workspace_bytes, void* stream, int impl);
 
-/* Workspace bytes of pdb_shared_prefix_attention for this shape (any kernel). */
+/* Workspace bytes of pdb_shared_prefix_attention for this shape (any kernel): about
+ * 8 * batch * tokens * heads * head_dim for partial sums and, with scores, 4 * batch *
+ * tokens * heads * max_length for logits. Give long prompts in several calls. */
 PDB_API size_t pdb_shared_prefix_attention_workspace_size(int64_t batch, int64_t tokens,
                                                           int64_t heads, int64_t kv_heads,
                                                           int64_t head_dim, int64_t prefix_length,

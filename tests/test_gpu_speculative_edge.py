@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from conftest import import_module
-from test_gpu_speculative import setup
+from oracle import llama_model as LM
+from test_gpu_speculative import dense, setup
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +76,47 @@ def test_a_failure_in_the_middle_changes_nothing(pkg, cuda, where, monkeypatch):
     batch.close()
     twin.close()
     assert pkg.read_device_errors() == 0
+
+
+def test_long_runs_are_scored_in_pieces(pkg, cuda, monkeypatch):
+    # logits, weights and steps as without pieces; no call takes more scratch than it may
+    module = import_module("speculative")
+    batches = [setup(pkg, torch.float32, budget=128, recent=8) for _ in range(2)]
+    (model, _, prefix, ids, batch, g), twin = batches[0], batches[1][4]
+    prompts = [torch.randint(0, 512, (n,), generator=g).tolist() for n in (120, 1, 47)]
+    drafts = [[3, 7, 5, 6, 2, 9], [8], []]
+    u, v = torch.zeros(3, 6, device=cuda), torch.full((3,), 0.7, device=cuda)
+    u[0, 4:] = 1.0  # four of six accepted
+    want = twin.score(prompts), twin.step([1, 2, 3], drafts, u, v)
+    sizes, real = [], module.shared_prefix_attention
+
+    def measured(q, *args, **kw):
+        out = real(q, *args, **kw)
+        scored = args[6] if kw.get("scores") is not None else 0
+        sizes.append((q.shape[1], 4 * q.shape[0] * q.shape[1] * q.shape[2] * (2 * q.shape[3] + scored)))
+        return out
+    limit = 4 * 3 * 4 * (2 * 64 + 130) * 3  # three tokens of 3 requests with 4 heads of 64
+    monkeypatch.setattr(module, "_SCRATCH", limit, raising=False)
+    monkeypatch.setattr(module, "shared_prefix_attention", measured)
+    got = batch.score(prompts)
+    assert max(size for _, size in sizes) <= limit and max(t for t, _ in sizes) > 1
+    for b, (rid, tokens) in enumerate(zip(ids, prompts)):
+        ref = dense(model, prefix + tokens)[-len(tokens):]
+        for logits in (got, want[0]):  # the runner's own bar
+            assert (logits[b, :len(tokens)] - ref).abs().max() <= 1e-5 * ref.abs().max()
+    assert batch.step([1, 2, 3], drafts, u, v) == want[1]
+    assert max(size for _, size in sizes) <= limit
+    assert batch.seen == twin.seen
+    torch.testing.assert_close(batch.scores, twin.scores, rtol=4e-5, atol=4e-6)
+    batch.close()
+    twin.close()
+
+
+def test_a_prompt_past_one_calls_tokens(pkg, cuda):
+    model = LM.seeded_model(LM.tiny_llama_config(), 3, torch.float32, "cuda")
+    runner = pkg.PagedLlama(model, blocks=300, block_size=16)
+    batch = pkg.PrefixBatch(runner, [5, 6, 7], ["a"], max_own=4300)
+    prompt = torch.randint(0, 512, (4200,), generator=torch.Generator().manual_seed(2)).tolist()
+    got, want = batch.score([prompt])[0], dense(model, [5, 6, 7] + prompt)[-4200:]
+    assert (got - want).abs().max() <= 1e-5 * want.abs().max()
+    batch.close()
