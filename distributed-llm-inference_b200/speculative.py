@@ -42,20 +42,28 @@ class PrefixBatch:
             raise ValueError("recent <= budget <= max_own is needed")
         self.runner, self.ids, self.max_own = runner, list(ids), max_own
         self.budget, self.recent, self.prefix_length = budget, recent, len(prefix)
-        cache = runner.cache
-        if prefix:
-            if not cache.reserve(_PREFIX, len(prefix)):
-                raise RuntimeError("the cache has no pages for the prefix")
-            runner.prefill([_PREFIX], [list(prefix)])
-        self.prefix_table = torch.tensor(cache.tables.get(_PREFIX, []), dtype=torch.int32,
-                                         device=runner.device)
-        for rid in self.ids:
-            if not cache.reserve(rid, max_own):
-                raise RuntimeError("the cache has no pages for the requests")
+        cache, mine = runner.cache, []
+
+        def reserve(rid, tokens, what):
+            if not cache.reserve(rid, tokens):
+                raise RuntimeError(f"the cache has no pages for the {what}")
+            mine.append(rid)
+        try:
+            if prefix:
+                reserve(_PREFIX, len(prefix), "prefix")
+                runner.prefill([_PREFIX], [list(prefix)])
+            self.prefix_table = torch.tensor(cache.tables.get(_PREFIX, []), dtype=torch.int32,
+                                             device=runner.device)
+            for rid in self.ids:
+                reserve(rid, max_own, "requests")
+            layers = len(runner.model.model.layers)
+            self.scores = torch.zeros((layers, len(self.ids), runner.kv_heads, max_own),
+                                      device=runner.device) if budget is not None else None
+        except BaseException:  # nothing stays reserved
+            for rid in mine:
+                cache.release(rid)
+            raise
         self.seen = {rid: 0 for rid in self.ids}  # own tokens so far, evicted ones included
-        layers = len(runner.model.model.layers)
-        self.scores = torch.zeros((layers, len(self.ids), runner.kv_heads, max_own),
-                                  device=runner.device) if budget is not None else None
 
     def close(self) -> None:
         for rid in [*self.ids, _PREFIX]:

@@ -1,0 +1,48 @@
+"""Host side of PrefixBatch (CPU): reservations, ids and refusals, on a runner without a model."""
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from conftest import import_module, import_pkg
+
+KV = import_module("paged_kv")
+
+
+class _Cfg:
+    num_hidden_layers, num_key_value_heads, head_dim = 2, 2, 8
+    num_attention_heads, hidden_size = 4, 32
+
+
+def fake_runner(blocks=40, vocab=512, fail=None):
+    cache = KV.DevicePagedKV(_Cfg, blocks=blocks, block_size=4, device="cpu", dtype=torch.float32,
+                             max_batch=8, max_tokens=160)
+
+    def prefill(ids, token_lists):
+        if fail is not None:
+            raise fail
+        for rid, tokens in zip(ids, token_lists):
+            cache.lengths[rid] = len(tokens)
+    inner = SimpleNamespace(layers=[None] * 2, embed_tokens=SimpleNamespace(num_embeddings=vocab))
+    return SimpleNamespace(cache=cache, prefill=prefill, device=torch.device("cpu"), heads=4, kv_heads=2,
+                           head_dim=8, model=SimpleNamespace(model=inner))
+
+
+@pytest.mark.parametrize("what, error", [
+    (dict(prefix=[1] * 156), RuntimeError),                        # no pages for the prefix
+    (dict(prefix=[1] * 20, max_own=80), RuntimeError),             # for one request, not for two
+    (dict(prefix=[1] * 20, ids=["a", "b", "a"]), ValueError),      # an id twice
+    (dict(prefix=[1] * 20, ids=["a", "taken"]), ValueError),       # somebody else's id
+    (dict(prefix=[1] * 20, fail=RuntimeError("out of memory")), RuntimeError),
+])
+def test_a_group_that_cannot_be_set_up_keeps_no_pages(what, error):
+    runner = fake_runner(fail=what.pop("fail", None))
+    runner.cache.reserve("taken", 10)
+    free, tables = sorted(runner.cache.free), dict(runner.cache.tables)
+    a = dict(prefix=[1, 2], ids=["a", "b"], max_own=20)
+    a.update(what)
+    with pytest.raises(error):
+        import_pkg().PrefixBatch(runner, a["prefix"], a["ids"], max_own=a["max_own"])
+    assert sorted(runner.cache.free) == free and runner.cache.tables == tables
