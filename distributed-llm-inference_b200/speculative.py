@@ -16,13 +16,14 @@ counted apart from its cache length.
 from __future__ import annotations
 
 import contextlib
+import itertools
 
 import torch
 
 from .ops import rope_kv_write
 from .serving_ops import evict_tokens, shared_prefix_attention, verify_drafts
 
-_PREFIX = "shared prefix"
+_groups = itertools.count()  # a number of its own for each PrefixBatch: its pages' ids
 
 # Bytes of scratch that one attention call may take, about (partial sums, and with scores
 # every row's logits over the own tokens, which grow with the square of a prompt):
@@ -42,32 +43,34 @@ class PrefixBatch:
             raise ValueError("recent <= budget <= max_own is needed")
         self.runner, self.ids, self.max_own = runner, list(ids), max_own
         self.budget, self.recent, self.prefix_length = budget, recent, len(prefix)
-        cache, mine = runner.cache, []
+        cache, self._reserved = runner.cache, []
+        prefix_id = ("shared prefix", next(_groups))
 
         def reserve(rid, tokens, what):
             if not cache.reserve(rid, tokens):
                 raise RuntimeError(f"the cache has no pages for the {what}")
-            mine.append(rid)
+            self._reserved.append(rid)
         try:
             if prefix:
-                reserve(_PREFIX, len(prefix), "prefix")
-                runner.prefill([_PREFIX], [list(prefix)])
-            self.prefix_table = torch.tensor(cache.tables.get(_PREFIX, []), dtype=torch.int32,
+                reserve(prefix_id, len(prefix), "prefix")
+                runner.prefill([prefix_id], [list(prefix)])
+            self.prefix_table = torch.tensor(cache.tables.get(prefix_id, []), dtype=torch.int32,
                                              device=runner.device)
             for rid in self.ids:
                 reserve(rid, max_own, "requests")
             layers = len(runner.model.model.layers)
             self.scores = torch.zeros((layers, len(self.ids), runner.kv_heads, max_own),
                                       device=runner.device) if budget is not None else None
-        except BaseException:  # nothing stays reserved
-            for rid in mine:
-                cache.release(rid)
+        except BaseException:
+            self.close()
             raise
         self.seen = {rid: 0 for rid in self.ids}  # own tokens so far, evicted ones included
 
     def close(self) -> None:
-        for rid in [*self.ids, _PREFIX]:
+        """Releases the pages that this group reserved (once)."""
+        for rid in self._reserved:
             self.runner.cache.release(rid)
+        self._reserved = []
 
     @contextlib.contextmanager
     def _unchanged_by_failure(self):

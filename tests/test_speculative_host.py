@@ -46,3 +46,34 @@ def test_a_group_that_cannot_be_set_up_keeps_no_pages(what, error):
     with pytest.raises(error):
         import_pkg().PrefixBatch(runner, a["prefix"], a["ids"], max_own=a["max_own"])
     assert sorted(runner.cache.free) == free and runner.cache.tables == tables
+
+
+def test_groups_on_one_cache_have_their_own_prefix():
+    runner = fake_runner()
+    cache, pkg = runner.cache, import_pkg()
+    one = pkg.PrefixBatch(runner, [1] * 10, ["a"], max_own=8)
+    two = pkg.PrefixBatch(runner, [2] * 6, ["b"], max_own=8)
+    none = pkg.PrefixBatch(runner, [], ["c"], max_own=8)
+    assert one.prefix_table.numel() == 3 and two.prefix_table.numel() == 2
+    assert none.prefix_table.numel() == 0 and none.prefix_length == 0
+    assert not set(one.prefix_table.tolist()) & set(two.prefix_table.tolist())
+    free = len(cache.free)
+    none.close()  # a group without a prefix releases nobody's
+    assert len(cache.free) == free + 2
+    two.close()
+    assert len(cache.free) == free + 6
+    assert not set(one.prefix_table.tolist()) & set(cache.free)
+    one.close()
+    assert len(cache.free) == 40 and not cache.tables
+
+
+def test_closing_twice_does_not_take_a_later_groups_requests():
+    runner = fake_runner()
+    first = import_pkg().PrefixBatch(runner, [1] * 10, ["a"], max_own=8)
+    first.close()
+    second = import_pkg().PrefixBatch(runner, [1] * 10, ["a"], max_own=8)
+    free = len(runner.cache.free)
+    first.close()
+    assert len(runner.cache.free) == free and "a" in runner.cache.tables
+    second.close()
+    assert len(runner.cache.free) == 40
