@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import contextlib
 import itertools
+import warnings
 
 import torch
 
@@ -35,7 +36,8 @@ class PrefixBatch:
     """Requests ``ids`` that continue ``prefix`` (token ids), up to ``max_own``
     cached own tokens each. With ``budget`` a request's own cache is cut to
     that many tokens per layer and kv head whenever a step left it longer; the
-    last ``recent`` stay in any case."""
+    last ``recent`` stay in any case. Pages for one request's budget are kept in
+    reserve for that; with more free pages more requests are cut at a time."""
 
     def __init__(self, runner, prefix, ids, max_own: int, budget: int | None = None,
                  recent: int = 32):
@@ -58,6 +60,10 @@ class PrefixBatch:
                                              device=runner.device)
             for rid in self.ids:
                 reserve(rid, max_own, "requests")
+            self._spare = None  # pages that the next request is cut into
+            if budget is not None and budget < max_own:
+                self._spare = (*prefix_id, "spare")
+                reserve(self._spare, budget, "eviction")
             layers = len(runner.model.model.layers)
             self.scores = torch.zeros((layers, len(self.ids), runner.kv_heads, max_own),
                                       device=runner.device) if budget is not None else None
@@ -201,8 +207,16 @@ class PrefixBatch:
         are. With a budget the attention runs a second time, over the tokens that
         stayed, for the weights that eviction goes by."""
         with self._unchanged_by_failure():
-            return self._step(last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs,
-                              temperature)
+            new = self._step(last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs,
+                             temperature)
+            over = [rid for rid in self.ids
+                    if self.budget is not None and self.runner.cache.lengths[rid] > self.budget]
+            over = over[self._evict_some(over):]
+        try:
+            self.evict(over)
+        except Exception as e:  # some are cut, so the step stands; the next one cuts the rest
+            warnings.warn(f"requests stay over their budget for a step: {e}")
+        return new
 
     def _step(self, last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs, temperature):
         cache, device = self.runner.cache, self.runner.device
@@ -225,21 +239,37 @@ class PrefixBatch:
             self.seen[rid] = seen[rid] + len(got)
         if self.budget is not None:
             self._accumulate(queries, [len(got) for got in new])
-            self.evict([rid for rid in self.ids if cache.lengths[rid] > self.budget])
         return new
 
     @torch.inference_mode()
     def evict(self, ids) -> None:
-        """Cuts the own caches of ``ids`` to the budget, into fresh pages."""
-        cache = self.runner.cache
-        ids = [rid for rid in ids if cache.reserve((rid, "kept"), self.max_own)]
-        if not ids:  # nothing to cut, or no free pages: the caches stay as they are
-            return
+        """Cuts the own caches of ``ids`` to the budget, into fresh pages, as many at a
+        time as there are pages for. Where it fails, those cut so far are cut and the
+        others as they were."""
+        if self._spare is None and ids:
+            raise ValueError("a group without a budget below max_own evicts nothing")
+        ids = list(ids)
+        while ids:
+            ids = ids[self._evict_some(ids):]
+
+    def _evict_some(self, ids) -> int:
+        """Cuts the first of ``ids``, and those after it that there are pages for;
+        returns how many. All of them or, where it fails, none."""
+        cache, reserved = self.runner.cache, []
+        if not ids:
+            return 0
         try:
+            into = {ids[0]: self._spare}
+            for rid in ids[1:]:
+                if not cache.reserve((rid, "kept"), self.budget):
+                    break
+                into[rid] = (rid, "kept")
+                reserved.append((rid, "kept"))
+            ids = list(into)
             rows = torch.tensor([self.ids.index(rid) for rid in ids], device=self.scores.device)
             tables, lengths, _ = cache.metadata(ids)
-            new_tables = torch.tensor([cache.tables[(rid, "kept")] for rid in ids],
-                                      dtype=torch.int32, device=tables.device)
+            new_tables = torch.tensor([cache.tables[into[rid]] for rid in ids], dtype=torch.int32,
+                                      device=tables.device)
             scores = self.scores.clone()
             for index in range(scores.shape[0]):
                 _, _, kept = evict_tokens(cache.keys[index], cache.values[index],
@@ -247,13 +277,15 @@ class PrefixBatch:
                                           self.budget, self.recent)
                 scores[index][rows] = kept
         except BaseException:
-            for rid in ids:
-                cache.release((rid, "kept"))
+            for rid in reserved:
+                cache.release(rid)
             raise
         self.scores = scores
-        for rid in ids:
-            length = min(cache.lengths[rid], self.budget)
-            pages = cache.tables[(rid, "kept")]
-            cache.tables[(rid, "kept")] = cache.tables[rid]
-            cache.release((rid, "kept"))
-            cache.tables[rid], cache.lengths[rid] = pages, length
+        for rid, other in into.items():
+            # the new pages, then what the old ones have beyond the budget: as many as before
+            new, old = cache.tables[other], cache.tables[rid]
+            cache.tables[rid], cache.tables[other] = new + old[len(new):], old[:len(new)]
+            cache.lengths[rid] = min(cache.lengths[rid], self.budget)
+            if other != self._spare:
+                cache.release(other)
+        return len(ids)

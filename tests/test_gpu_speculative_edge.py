@@ -120,3 +120,64 @@ def test_a_prompt_past_one_calls_tokens(pkg, cuda):
     got, want = batch.score([prompt])[0], dense(model, [5, 6, 7] + prompt)[-4200:]
     assert (got - want).abs().max() <= 1e-5 * want.abs().max()
     batch.close()
+
+
+def test_a_full_cache_still_evicts(pkg, cuda):
+    # no free pages but those in reserve: the same tokens, scores and lengths as with room
+    prefix = torch.randint(0, 512, (75,), generator=torch.Generator().manual_seed(5)).tolist()
+    results = []
+    for spare in (0, 2, 300):  # pages beyond the prefix's 5, the requests' 3 x 6 and the reserve's 2
+        model = LM.seeded_model(LM.tiny_llama_config(), 3, torch.float32, "cuda")
+        runner = pkg.PagedLlama(model, blocks=5 + 18 + 2 + spare, block_size=16)
+        batch = pkg.PrefixBatch(runner, prefix, ["a", "b", "c"], max_own=90, budget=24, recent=8)
+        free = len(runner.cache.free)
+        assert free == spare
+        g = torch.Generator().manual_seed(1)
+        last, out = [1, 2, 3], []
+        for _ in range(25):
+            u, v = torch.rand(3, 3, generator=g).cuda(), torch.rand(3, generator=g).cuda()
+            new = batch.step(last, [[5, 9, 11]] * 3, u, v)
+            last = [n[-1] for n in new]
+            out.append((new, batch.scores.clone()))
+            assert max(runner.cache.lengths[r] for r in "abc") <= 24
+            pages = [p for t in runner.cache.tables.values() for p in t] + runner.cache.free
+            assert sorted(pages) == list(range(runner.cache.total_blocks))  # each in one place
+            assert [len(runner.cache.tables[r]) for r in "abc"] == [6, 6, 6]
+            assert len(runner.cache.free) == free
+        results.append(out)
+        batch.close()
+        assert len(runner.cache.free) == runner.cache.total_blocks
+    for other in results[1:]:
+        for (new, scores), (new2, scores2) in zip(results[0], other):
+            assert new == new2 and torch.equal(scores, scores2)
+    assert pkg.read_device_errors() == 0
+
+
+def test_a_later_cut_that_fails_waits_for_the_next_step(pkg, cuda, monkeypatch):
+    module = import_module("speculative")
+    prefix = [4] * 20
+    batches = []
+    for _ in range(2):
+        model = LM.seeded_model(LM.tiny_llama_config(), 3, torch.float32, "cuda")
+        runner = pkg.PagedLlama(model, blocks=2 + 6 + 1, block_size=16)
+        batches.append(pkg.PrefixBatch(runner, prefix, ["a", "b"], max_own=40, budget=16, recent=4))
+        batches[-1].score([[i % 7 for i in range(15)], [i % 5 for i in range(15)]])
+    batch, twin = batches
+    u, v = torch.zeros(2, 2, device=cuda), torch.full((2,), 0.3, device=cuda)
+    real, left = module.evict_tokens, [2]  # two layers of the first request
+
+    def failing(*args):
+        left[0] -= 1
+        if left[0] < 0:
+            raise RuntimeError("out of memory")
+        return real(*args)
+    with monkeypatch.context() as m:
+        m.setattr(module, "evict_tokens", failing)
+        with pytest.warns(UserWarning, match="over their budget"):
+            got = batch.step([7, 8], [[1, 2]] * 2, u, v)
+    assert got == twin.step([7, 8], [[1, 2]] * 2, u, v)
+    assert batch.runner.cache.lengths["a"] == 16 and batch.runner.cache.lengths["b"] == 18
+    assert batch.seen == twin.seen and torch.equal(batch.scores[:, 0], twin.scores[:, 0])
+    batch.evict(["b"])
+    assert batch.runner.cache.lengths["b"] == 16 and torch.equal(batch.scores, twin.scores)
+    assert batch.step([7, 8], [[1, 2]] * 2, u, v) == twin.step([7, 8], [[1, 2]] * 2, u, v)

@@ -77,3 +77,21 @@ def test_closing_twice_does_not_take_a_later_groups_requests():
     assert len(runner.cache.free) == free and "a" in runner.cache.tables
     second.close()
     assert len(runner.cache.free) == 40
+
+
+def test_a_budget_needs_pages_to_evict_into():
+    # prefix 3 pages, two requests of 10; the budget needs 5 too
+    pkg = import_pkg()
+    runner = fake_runner(blocks=27)
+    with pytest.raises(RuntimeError, match="no pages for the eviction"):
+        pkg.PrefixBatch(runner, [1] * 10, ["a", "b"], max_own=40, budget=20, recent=4)
+    assert len(runner.cache.free) == 27
+    runner = fake_runner(blocks=28)
+    batch = pkg.PrefixBatch(runner, [1] * 10, ["a", "b"], max_own=40, budget=20, recent=4)
+    assert not runner.cache.free
+    batch.close()
+    assert len(runner.cache.free) == 28
+    whole = fake_runner(blocks=23)  # nothing can pass this budget
+    pkg.PrefixBatch(whole, [1] * 10, ["a", "b"], max_own=40, budget=40).close()
+    with pytest.raises(ValueError, match="evicts nothing"):
+        pkg.PrefixBatch(whole, [1] * 10, ["a", "b"], max_own=40).evict(["a"])
