@@ -41,8 +41,10 @@ class PrefixBatch:
 
     def __init__(self, runner, prefix, ids, max_own: int, budget: int | None = None,
                  recent: int = 32):
-        if budget is not None and not 0 <= recent <= budget <= max_own:
+        if budget is not None and not (0 <= recent <= budget <= max_own and budget > 0):
             raise ValueError("recent <= budget <= max_own is needed")
+        self.vocab = runner.model.model.embed_tokens.num_embeddings
+        self._check_tokens(prefix)
         self.runner, self.ids, self.max_own = runner, list(ids), max_own
         self.budget, self.recent, self.prefix_length = budget, recent, len(prefix)
         cache, self._reserved = runner.cache, []
@@ -78,6 +80,11 @@ class PrefixBatch:
             self.runner.cache.release(rid)
         self._reserved = []
 
+    def _check_tokens(self, tokens) -> None:
+        # an index outside the embedding is a fault on the GPU
+        if not all(0 <= t < self.vocab for t in tokens):
+            raise ValueError("token outside the vocabulary")
+
     @contextlib.contextmanager
     def _unchanged_by_failure(self):
         """What fails inside (no memory, a refused argument) leaves the requests as they
@@ -111,6 +118,10 @@ class PrefixBatch:
         """``score``; with ``queries`` each layer's rotated queries are added to that
         list, and no weights to the scores."""
         lengths, counts = self.runner.cache.lengths, [len(tokens) for tokens in token_lists]
+        if len(counts) != len(self.ids):
+            raise ValueError("each request needs its tokens")
+        for tokens in token_lists:
+            self._check_tokens(tokens)
         after = [lengths[rid] + n for rid, n in zip(self.ids, counts)]
         if any(not n for n in counts) or max(after) > self.max_own:
             raise ValueError("each request takes one token at least, and max_own cached in all")
@@ -220,6 +231,13 @@ class PrefixBatch:
 
     def _step(self, last_tokens, drafts, accept_uniforms, sample_uniforms, draft_probs, temperature):
         cache, device = self.runner.cache, self.runner.device
+        if not 0.0 < temperature < float("inf"):
+            raise ValueError("the temperature must be positive and finite")
+        if not len(last_tokens) == len(drafts) == len(self.ids):
+            raise ValueError("each request needs its last token and its drafts")
+        if accept_uniforms.dim() != 2 or accept_uniforms.shape[0] != len(self.ids) or any(
+                len(d) > accept_uniforms.shape[1] for d in drafts):
+            raise ValueError("accept_uniforms needs a row per request, a number per draft")
         T = accept_uniforms.shape[1]
         before = [cache.lengths[rid] for rid in self.ids]
         seen = dict(self.seen)
@@ -233,6 +251,8 @@ class PrefixBatch:
             probs.contiguous(), accept_uniforms, sample_uniforms, draft_probs=draft_probs,
             draft_lengths=torch.tensor([len(d) for d in drafts], dtype=torch.int32, device=device))
         new = [row[:n] for row, n in zip(tokens.tolist(), counts.tolist())]
+        if any(t < 0 for got in new for t in got):
+            raise RuntimeError("the model's probabilities leave no token to draw (NaN logits?)")
         for b, (rid, got) in enumerate(zip(self.ids, new)):
             # the last token and the accepted drafts stay cached; cells past them are free
             cache.lengths[rid] = before[b] + len(got)

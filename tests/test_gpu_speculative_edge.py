@@ -181,3 +181,22 @@ def test_a_later_cut_that_fails_waits_for_the_next_step(pkg, cuda, monkeypatch):
     batch.evict(["b"])
     assert batch.runner.cache.lengths["b"] == 16 and torch.equal(batch.scores, twin.scores)
     assert batch.step([7, 8], [[1, 2]] * 2, u, v) == twin.step([7, 8], [[1, 2]] * 2, u, v)
+
+
+def test_logits_that_are_not_numbers_end_the_step(pkg, cuda, monkeypatch):
+    _, runner, _, ids, batch, g = setup(pkg, torch.float32, budget=64, recent=8)
+    batch.score([[1, 2], [3], [4, 5, 6]])
+    before = dict(runner.cache.lengths), dict(batch.seen), batch.scores.clone()
+    u, v = torch.rand(3, 2, generator=g).cuda(), torch.rand(3, generator=g).cuda()
+    head = runner.model.lm_head
+    nan = torch.nn.Module()
+    nan.forward = lambda x: head(x) * float("nan")
+    monkeypatch.setattr(runner.model, "lm_head", nan)
+    with pytest.raises(RuntimeError, match="no token to draw"):
+        batch.step([7, 8, 9], [[1, 2], [], [3]], u, v)
+    assert before[:2] == (runner.cache.lengths, batch.seen) and torch.equal(before[2], batch.scores)
+    monkeypatch.setattr(runner.model, "lm_head", head)
+    new = batch.step([7, 8, 9], [[1, 2], [], [3]], u, v)
+    assert all(0 <= t < 512 for got in new for t in got)
+    batch.close()
+    assert pkg.read_device_errors() == 0

@@ -95,3 +95,37 @@ def test_a_budget_needs_pages_to_evict_into():
     pkg.PrefixBatch(whole, [1] * 10, ["a", "b"], max_own=40, budget=40).close()
     with pytest.raises(ValueError, match="evicts nothing"):
         pkg.PrefixBatch(whole, [1] * 10, ["a", "b"], max_own=40).evict(["a"])
+
+
+def unchanged(runner, batch, call, error=ValueError, match=None):
+    before = dict(runner.cache.lengths), dict(batch.seen), sorted(runner.cache.free)
+    with pytest.raises(error, match=match):
+        call()
+    assert before == (runner.cache.lengths, batch.seen, sorted(runner.cache.free))
+
+
+def test_refusals_before_anything_is_computed():
+    # the runner has no layers: a call that got further than its checks would fail otherwise
+    runner = fake_runner(vocab=100)
+    batch = import_pkg().PrefixBatch(runner, [1] * 10, ["a", "b"], max_own=8)
+    for lists in ([[100], [1]], [[1], [-1]], [[1]], [[1], [2], [3]], [[], [1]], [[1] * 9, [1]]):
+        unchanged(runner, batch, lambda: batch.score(lists))
+    u, v = torch.rand(2, 3), torch.rand(2)
+    good = dict(last=[1, 2], drafts=[[3, 4], []], u=u, v=v, temperature=1.0)
+
+    def step(**kw):
+        a = dict(good, **kw)
+        return lambda: batch.step(a["last"], a["drafts"], a["u"], a["v"], temperature=a["temperature"])
+    for kw, match in [
+            (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"),
+            (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"),
+            (dict(drafts=[[1, 2, 3, 4], []]), "accept_uniforms"), (dict(drafts=[[3, 100], []]), "vocabulary"),
+            (dict(drafts=[[-1], []]), "vocabulary"), (dict(last=[-1, 2]), "vocabulary"),
+            (dict(last=[1]), "each request"), (dict(drafts=[[1]]), "each request"),
+            (dict(u=torch.rand(3, 3)), "accept_uniforms"), (dict(u=torch.rand(2)), "accept_uniforms")]:
+        unchanged(runner, batch, step(**kw), match=match)
+    for prefix, kw in (([1, 100], {}), ([-1], {}), ([1], dict(budget=0, recent=0))):
+        with pytest.raises(ValueError):
+            import_pkg().PrefixBatch(runner, prefix, ["c"], max_own=8, **kw)
+    batch.close()
+    assert len(runner.cache.free) == 40
