@@ -8,8 +8,8 @@
 // probabilities: p_a with x_a taken out), from p_n when all were accepted.
 // The drawing inverts the running sum of W_j = floor(min(w_j, 1) 2^40) at
 // floor(u sum W): the W_j are 64-bit integers, so their sums are exact and the
-// token does not depend on how the vocabulary is split over threads (at most
-// 2^23 entries of 2^40 each stay far below 2^63; a weight below 2^-40 counts
+// token does not depend on how the vocabulary is split over threads (the at most
+// 2^22 entries of 2^40 each stay below 2^63; a weight below 2^-40 counts
 // as none). A row whose w are all zero (p_a = q_a up to rounding) falls back
 // to p_a; a row without any weight gives token -1.
 //

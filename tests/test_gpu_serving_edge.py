@@ -14,7 +14,7 @@ import torch
 
 import serving_oracle as oracle
 from conftest import import_module
-from test_gpu_serving_ops import IMPLS, TOL, call, impl_of, make
+from test_gpu_serving_ops import IMPLS, TOL, call, drafts, impl_of, make, verify
 
 pytestmark = pytest.mark.gpu
 
@@ -237,3 +237,66 @@ def test_accumulated_weights_of_very_many_heads(pkg, cuda):
         _, half = call(pkg, dict(d, **{n: d[n][part] for n in ("q", "tables", "lengths", "scores")}), cuda)
         torch.testing.assert_close(scores[part], half, rtol=4e-5, atol=4e-6)
     assert pkg.read_device_errors() == 0
+
+
+# ---- paths that only large calls take ------------------------------------------------
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B, T, own", [(621, 1, 0), (297, 4, 9)])
+def test_tcgen05_ranges_that_cross_items(pkg, cuda, B, T, own, D):
+    # 80 and 152 pairs of query tiles, 4 key tiles each, cut into one range per CTA: most
+    # CTAs work on the end of one pair and the start of the next. The last pair is not full, the
+    # prefix ends inside a tile.
+    lengths = [T + b % (own - T + 1) if own else 0 for b in range(B)]
+    d = make(B, T, 32, 8, D, torch.float16, 500, lengths)
+    got, beside = (call(pkg, d, cuda, impl).cpu().double() for impl in ("tcgen05", "mma"))
+    some = [0, 1, 15, 16, 17, B // 3, B // 2, B - 18, B - 17, B - 2, B - 1]
+    want, _ = oracle.shared_prefix_attention(d["q"][some], d["k"], d["v"], d["prefix_table"], 500,
+                                             d["tables"][some], d["lengths"][some])
+    top = d["v"][d["v"] == d["v"]].abs().max().item()
+    assert (got[some] - want).abs().max().item() <= TOL[torch.float16] * top
+    assert (got - beside).abs().max().item() <= 2 * TOL[torch.float16] * top  # every row
+    assert pkg.read_device_errors() == 0
+
+
+@pytest.mark.parametrize("B, V, dtype, given", [
+    (300, 140011, torch.float16, False), (300, 140011, torch.float16, True),
+    (1, 8 * 131072 + 1003, torch.float32, True), (1, 1 << 22, torch.float16, False)])
+def test_verify_blocks_of_several_rounds(pkg, cuda, B, V, dtype, given):
+    # more than 512 blocks of 256 entries per CTA: blocks of 512 and up to 1024 entries
+    g = torch.Generator(device=cuda).manual_seed(V)
+    target = torch.rand(B, 2, V, generator=g, device=cuda).pow_(4)
+    target = target.div_(target.sum(-1, keepdim=True)).mul_(3000 if dtype == torch.float16 else 1).to(dtype)
+    draft = target[:, :1].flip(-1).contiguous() if given else None
+    tokens = torch.randint(0, V, (B, 1), generator=g, device=cuda)
+    accept, sample = (torch.rand(s, generator=g, device=cuda) for s in ((B, 1), (B,)))
+    sample[:3] = torch.tensor([0.0, 1 - 2.0 ** -24, 0.999])[:B].to(cuda)
+    got, counts = pkg.verify_drafts(tokens, target, accept, sample, draft_probs=draft)
+    some = [b for b in (0, 1, 2, 3, 150, 299) if b < B]
+    want, want_counts = oracle.verify_drafts(
+        tokens[some].cpu(), target[some].cpu(), accept[some].cpu(), sample[some].cpu(),
+        draft[some].cpu() if given else None)
+    assert torch.equal(got.cpu()[some], want) and torch.equal(counts.cpu()[some], want_counts)
+    assert pkg.read_device_errors() == 0
+
+
+@pytest.mark.parametrize("given", [True, False])
+def test_verified_tokens_follow_the_target(pkg, cuda, given):
+    # what the rule is for: whatever was drafted, the tokens are the target's. 40000 trials;
+    # chi-square with 6 degrees of freedom is above 36 with probability 3e-6
+    B, V = 40000, 7
+    g = torch.Generator().manual_seed(8)
+    p = torch.softmax(torch.randn(3, V, generator=g), -1)
+    q = torch.softmax(torch.randn(2, V, generator=g), -1)
+    tokens = torch.stack([torch.multinomial(q[i], B, replacement=True, generator=g) for i in range(2)], 1)
+    if not given:
+        tokens = torch.tensor([2, 5]).expand(B, 2).contiguous()
+    out, counts = verify(pkg, dict(
+        draft_tokens=tokens, target=p.expand(B, 3, V).contiguous(),
+        draft=q.expand(B, 2, V).contiguous() if given else None,
+        accept=torch.rand(B, 2, generator=g), sample=torch.rand(B, generator=g), draft_lengths=None), cuda)
+    for place in range(3):
+        there = out[counts > place, place]
+        expected = p[place].double() * len(there)
+        assert expected.min() > 5  # what the chi-square approximation asks for
+        seen = torch.bincount(there, minlength=V).double()
+        assert ((seen - expected) ** 2 / expected).sum() < 36
