@@ -24,11 +24,11 @@
 //     The MMAs of a CTA run in issue order, so S_{j+1} may overwrite P_j
 //     without a barrier, and the commit that publishes S_{j+1} also says that
 //     O holds P_j V_j (what a rescale needs).
-// Measured on 4096 rows x 8192 keys x 8 heads, 128 dims: 168 us, 0.82 PFLOP/s of the formula's
-// operations and half as many again for the second term of P (137 us without it).
-// Handing P over in halves (the product of one while the other is exponentiated) or
-// reading the logits a quarter ahead were slower (190 to 200 against 178 with the join), as was
-// rounding the first term and converting it back (190).
+// Measured on 4096 rows x 8192 keys x 8 heads, 128 dims: 178 us with the join, 0.77 PFLOP/s
+// of the formula's operations and half as many again for the second term of P (147 us without
+// it); tensor pipe 65% busy. Handing P over in halves (the product of one while the other is exponentiated) or
+// reading the logits a quarter ahead were slower (190 to 200), as was rounding the first term
+// and converting it back (190).
 // TMEM: S0 S1 O0 O1, 128 columns each = all 512.
 // Query rows: a tile holds floor(128 / G) tokens with all G heads of the kv
 // head, one TMA box {64 columns, G heads, floor(128 / G) tokens}, so any group
