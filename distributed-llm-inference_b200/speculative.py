@@ -100,12 +100,14 @@ class PrefixBatch:
             raise
 
     @torch.inference_mode()
-    def score(self, token_lists) -> torch.Tensor:
+    def score(self, token_lists, last_only: bool = False) -> torch.Tensor:
         """Appends each request's tokens (one or more, ragged) to its cache and
         returns the logits that follow them, float32 [B, T, vocab] (rows past a
-        request's own count are meaningless)."""
+        request's own count are meaningless). With ``last_only`` the LM head runs
+        on each request's last token alone, and its logits are returned,
+        [B, vocab]: for prompts, whose other logits nobody reads."""
         with self._unchanged_by_failure():
-            return self._score(token_lists)
+            return self._score(token_lists, last_only=last_only)
 
     def _piece(self, longest: int, scored: bool) -> int:
         """Tokens per request that one attention call takes."""
@@ -114,7 +116,10 @@ class PrefixBatch:
                                                         + (longest if scored else 0))
         return max(1, min(4096, _SCRATCH // per_token))  # 4096: the operator's own limit
 
-    def _score(self, token_lists, queries: list | None = None) -> torch.Tensor:
+    def _logits(self, hidden: torch.Tensor) -> torch.Tensor:
+        return self.runner.model.lm_head(hidden).float()
+
+    def _score(self, token_lists, queries: list | None = None, last_only: bool = False):
         """``score``; with ``queries`` each layer's rotated queries are added to that
         list, and no weights to the scores."""
         lengths, counts = self.runner.cache.lengths, [len(tokens) for tokens in token_lists]
@@ -126,22 +131,28 @@ class PrefixBatch:
         if any(not n for n in counts) or max(after) > self.max_own:
             raise ValueError("each request takes one token at least, and max_own cached in all")
         T, size = max(counts), self._piece(max(after), queries is None and self.scores is not None)
-        if T <= size:
-            return self._forward(token_lists, queries)
-        logits, kept = None, []
+        out, kept = None, []
         for t0 in range(0, T, size):
             piece, kept_here = [tokens[t0:t0 + size] for tokens in token_lists], []
-            part = self._forward(piece, None if queries is None else kept_here)
-            if logits is None:
-                logits = part.new_empty((part.shape[0], T, part.shape[2]))
-            logits[:, t0:t0 + size] = part
+            hidden = self._forward(piece, None if queries is None else kept_here)
             kept.append(kept_here)
+            if last_only:  # the hidden states of the last tokens, from the pieces they are in
+                ends = [b for b, n in enumerate(counts) if t0 < n <= t0 + size]
+                out = hidden.new_empty((len(counts), hidden.shape[2])) if out is None else out
+                out[ends] = hidden[ends, [counts[b] - 1 - t0 for b in ends]]
+            elif T <= size:
+                out = self._logits(hidden)
+            else:
+                part = self._logits(hidden)
+                out = part.new_empty((part.shape[0], T, part.shape[2])) if out is None else out
+                out[:, t0:t0 + size] = part
         if queries is not None:
-            queries += [torch.cat(parts, 1) for parts in zip(*kept)]
-        return logits
+            queries += [torch.cat(parts, 1) for parts in zip(*kept)] if len(kept) > 1 else kept[0]
+        return self._logits(out) if last_only else out
 
     def _forward(self, token_lists, queries: list | None) -> torch.Tensor:
-        """One pass over the layers; requests may have no token in it."""
+        """One pass over the layers, to the normed hidden states [B, T, hidden]; requests
+        may have no token in it."""
         runner, cache = self.runner, self.runner.cache
         counts = [len(tokens) for tokens in token_lists]
         B, T = len(self.ids), max(counts)
@@ -179,7 +190,7 @@ class PrefixBatch:
             x = x + layer.mlp(layer.post_attention_layernorm(x))
         if scores is not None:
             self.scores = new_scores
-        return runner.model.lm_head(runner.model.model.norm(x)).float()
+        return runner.model.model.norm(x)
 
     @staticmethod
     def _scored(scores, new_scores, index) -> dict:

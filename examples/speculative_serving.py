@@ -45,7 +45,8 @@ def main():
     ids = [f"request {i}" for i in range(args.requests)]
     text = {rid: torch.randint(0, 512, (12,), generator=g).tolist() for rid in ids}
     batch = b200.PrefixBatch(runner, prefix, ids, max_own=512, budget=args.budget, recent=16)
-    batch.score([text[rid][:-1] for rid in ids])  # the requests' own prompts, all but the last token
+    # the requests' own prompts, all but the last token; their logits are not needed
+    batch.score([text[rid][:-1] for rid in ids], last_only=True)
     made = 0
     for _ in range(args.steps):
         drafts = [look_up(text[rid], args.drafts) for rid in ids]

@@ -200,3 +200,25 @@ def test_logits_that_are_not_numbers_end_the_step(pkg, cuda, monkeypatch):
     assert all(0 <= t < 512 for got in new for t in got)
     batch.close()
     assert pkg.read_device_errors() == 0
+
+
+@pytest.mark.parametrize("pieces", [False, True])
+def test_last_logits_alone(pkg, cuda, pieces, monkeypatch):
+    batches = [setup(pkg, torch.float32, budget=128, recent=8) for _ in range(2)]
+    (_, runner, _, _, batch, g), twin = batches[0], batches[1][4]
+    prompts = [torch.randint(0, 512, (n,), generator=g).tolist() for n in (50, 1, 47)]
+    want = twin.score(prompts)
+    if pieces:
+        monkeypatch.setattr(import_module("speculative"), "_SCRATCH", 4 * 3 * 4 * (2 * 64 + 60) * 7)
+    rows = []
+    hook = runner.model.lm_head.register_forward_pre_hook(lambda m, a: rows.append(a[0].shape[:-1].numel()))
+    got = batch.score(prompts, last_only=True)
+    hook.remove()
+    assert rows == [3] and got.shape == (3, 512) and got.dtype == torch.float32
+    last = torch.stack([want[b, len(p) - 1] for b, p in enumerate(prompts)])
+    # both within the runner's own bar of the dense model
+    assert (got - last).abs().max() <= 2e-5 * last.abs().max()
+    assert batch.seen == twin.seen
+    torch.testing.assert_close(batch.scores, twin.scores, rtol=4e-5, atol=4e-6)
+    batch.close()
+    twin.close()
